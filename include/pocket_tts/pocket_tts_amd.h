@@ -3,7 +3,7 @@
  * pocket_tts_c.h; these calls expose (1) options the reference can only set from C++ or its CLI,
  * (2) a batch ingress for many independent utterances, and (3) one entry point per ONNX Runtime
  * call site of the reference so each network can be checked in isolation.  All buffers are host
- * memory; sizes are in elements.  Return value 0 = success, -1 = failure with the message available
+ * memory unless stated otherwise; sizes are in elements.  Return value 0 = success, -1 = failure with the message available
  * from pocket_tts_get_last_error(), unless stated otherwise.
  */
 #ifndef POCKET_TTS_AMD_H
@@ -139,6 +139,110 @@ POCKET_TTS_API int ptts_mimi_encode(PocketTTSHandle handle, const float* audio, 
  * most cap_frames of them, as above). */
 POCKET_TTS_API int ptts_mimi_encode_batch(PocketTTSHandle handle, const float* const* clips, int n_clips, int samples, float* const* outs,
                                           int cap_frames);
+
+/* ---- keys and values in pages: plan, rotary append, attention ------------------------------------------------------------
+ *
+ * For serving loops that schedule by themselves: requests share a pool of pages instead of holding a slot of fixed length each
+ * (ptts_state_new), so one voice's rows serve many utterances, prompts arrive in chunks and long streams keep a window.
+ * One step of a model calls ptts_paged_plan once, then ptts_rotary_append and ptts_paged_attention for every layer.
+ *
+ * Unlike the calls above, these take DEVICE pointers of GPU `device`, enqueue on `stream` (a hipStream_t; NULL: the device's
+ * default stream) and return without waiting: 0, or -1 with a message and nothing launched.  They allocate nothing, keep nothing
+ * between calls, may be called from several threads at once and may be captured into a graph.  Buffers must not overlap unless
+ * stated.  Strides count elements; the last axis is contiguous.  Values in device memory (lengths, page ids, slots) are checked
+ * by the kernels: what is out of range is not read or written and sets a bit of *status (may be NULL; the caller clears it):
+ * 1 page id or slot outside the pool, 2 row ranges outside the rows or not ascending, 4 a length negative or beyond its table. */
+enum { PTTS_TYPE_F32 = 0, PTTS_TYPE_BF16 = 1, PTTS_TYPE_F16 = 2 };
+
+/* A pool of pages: key row r of page p and head h at k + p * page_stride + r * row_stride + h * head_stride, values likewise at v.
+ * Pointers and strides are multiples of 16 bytes, head_dim is a multiple of 8 up to 256; any page_size, pages * page_size < 2^30. */
+typedef struct {
+    void* k;
+    void* v;
+    long long page_stride, row_stride, head_stride;
+    int type, pages, page_size, kv_heads, head_dim;
+} PttsPages;
+
+/* Block tables and slot maps from request lengths, in one launch.  Request i holds cached[i] rows in the first
+ * ceil(cached[i] / page_size) pages of its block_table row and receives arriving[i] more.  The pages it lacks are taken from
+ * free_pages in order (request 0's first) and entered in its table row; other entries stay as they are.  Row r of the packed new
+ * rows (request 0's first) gets positions[r] and slot_map[r] = page * page_size + row inside the page.  cu_rows[i] is the first
+ * packed row of request i (requests + 1 entries), kv_len[i] = cached[i] + arriving[i].
+ * counts[4] = new rows in all (those beyond `rows` are not written), pages taken, pages missing, rows without a page.  A page that is missing (free list exhausted, or
+ * table row full) leaves -1 in the table and its rows get slot -1.  A negative length counts as 0.
+ * Rows of slot_map and positions behind the last new row stay as they are.  The last page of a request must not be shared when
+ * it is partly filled and rows arrive.  requests <= 65536. */
+typedef struct {
+    const int* cached;
+    const int* arriving;
+    const int* free_pages;
+    int* block_table;
+    int* slot_map;
+    int* positions;
+    int* cu_rows;
+    int* kv_len;
+    int* counts;
+    int* status;
+    long long table_stride;
+    int requests, table_width, n_free, page_size, rows;
+} PttsPagedPlan;
+POCKET_TTS_API int ptts_paged_plan(const PttsPagedPlan* plan, int device, void* stream);
+
+/* Rotary frequencies for ptts_rotary_append, on the host: out[rot_dim / 2] in radians per position; *magnitude (may be NULL) is the
+ * factor for the rotated values.  scaling 0: base^(-2 i / rot_dim).  1: positions divided by `factor`.  2: the base stretched so
+ * that the lowest frequency is divided by `factor` and the highest kept.  3: by parts: frequencies that turn more than `fast`
+ * times within `trained` positions are kept, those below `slow` turns are divided by `factor`, a linear ramp in between, and
+ * magnitude = 0.1 ln(factor) + 1. */
+POCKET_TTS_API int ptts_rotary_frequencies(int rot_dim, double base, int scaling, double factor, double trained, double fast, double slow,
+                                           double* out, float* magnitude);
+
+/* Rotates the first rot_dim values of every head of q and k by positions[row] * freq[i] (device, float64: far positions keep their
+ * angle), pairs (2 i, 2 i + 1) if interleaved, else (i, i + rot_dim / 2), times `magnitude`; the rest of the head passes unscaled.  q goes to q_out (q itself
+ * is allowed, with the same strides).  k and v go to the pages, row r to slot slot_map[r] (-1: not stored).  Two rows must not
+ * name one slot.  q, or k and v (then pages and slot_map too), may be NULL.  q, q_out, k and v have `type`; the pages
+ * have the same, or bf16 under f32 rows (rounded to nearest even). */
+typedef struct {
+    const void* q;
+    const void* k;
+    const void* v;
+    void* q_out;
+    const int* positions;
+    const int* slot_map;
+    const double* freq;
+    int* status;
+    long long q_row_stride, q_head_stride, k_row_stride, k_head_stride, v_row_stride, v_head_stride, out_row_stride, out_head_stride;
+    PttsPages pages;   /* without k and v only head_dim is read */
+    float magnitude;
+    int type, rows, q_heads, rot_dim, interleaved;
+} PttsRotaryAppend;
+POCKET_TTS_API int ptts_rotary_append(const PttsRotaryAppend* args, int device, void* stream);
+
+/* Attention of every request's new rows over its pages.  Rows cu_rows[i] .. cu_rows[i + 1] - 1 of q are request i's last positions,
+ * kv_len[i] - 1 for the last of them (so their own keys are in the pages already).  The query at position p sees key j if j <= p and
+ * (window <= 0 or j > p - window or j < sinks).  out = softmax(scale q.k) v, lse (may be NULL) = ln sum exp(scale q.k); a row that
+ * sees nothing gets 0 and -inf.  Head h of q reads head h / (q_heads / kv_heads) of the pages.  Keys that a row does not see
+ * never reach it, whatever they hold.  out may not alias q.
+ * Types: q and out q_type; pages of q_type, or bf16 pages under f32 rows.  Rows outside every request stay as they were.
+ * max_rows, max_kv: what the caller knows of the largest row count and length of a request (0: nothing).  They choose how the work
+ * is cut and cost time when wrong, never results.
+ * workspace: ptts_paged_attention_workspace() bytes (0: none needed; -1: bad arguments), 16-byte aligned, contents irrelevant
+ * before and after; concurrent calls (and graphs that may run at the same time) need one each. */
+typedef struct {
+    const void* q;
+    void* out;
+    float* lse;
+    const int* cu_rows;
+    const int* kv_len;
+    const int* block_table;
+    int* status;
+    void* workspace;
+    long long q_row_stride, q_head_stride, out_row_stride, out_head_stride, lse_row_stride, table_stride, workspace_bytes;
+    PttsPages pages;
+    float scale;
+    int q_type, rows, requests, q_heads, table_width, window, sinks, max_rows, max_kv;
+} PttsPagedAttention;
+POCKET_TTS_API long long ptts_paged_attention_workspace(const PttsPagedAttention* args, int device);
+POCKET_TTS_API int ptts_paged_attention(const PttsPagedAttention* args, int device, void* stream);
 
 /* ---- host-side pre/post steps, usable without a GPU ---------------------------------------------- */
 

@@ -2,6 +2,7 @@
 // additive ones of pocket_tts_amd.h.  Conventions follow /root/reference/src/pocket_tts_c.cpp:
 // exceptions never cross the boundary, failures set a thread-local message (:11, :23-25, :159-161).
 #include <algorithm>
+#include <atomic>
 #include <cstring>
 #include <exception>
 #include <string>
@@ -10,6 +11,7 @@
 
 #include "onnx_reader.h"
 #include "engine.h"
+#include "paged.h"
 #include "pocket_tts/audio_utils.hpp"
 #include "pocket_tts/pocket_tts.hpp"
 #include "pocket_tts/pocket_tts_amd.h"
@@ -656,6 +658,91 @@ POCKET_TTS_API int ptts_weight_bytes(PocketTTSHandle handle, unsigned long long*
 }
 
 }  // extern "C"
+
+// ------------------------------------------------------------------ keys and values in pages (device pointers, caller's stream)
+
+namespace {
+
+// The caller's current device back when the call ends, whatever happens in between.
+struct OnDevice {
+    int before = -1;
+    explicit OnDevice(int device) {
+        int n = 0;
+        if (hipGetDeviceCount(&n) != hipSuccess || n == 0) throw std::runtime_error("no HIP device");
+        if (device < 0 || device >= n) throw std::runtime_error("device " + std::to_string(device) + " of " + std::to_string(n));
+        PTTS_HIP(hipGetDevice(&before));
+        if (before != device) PTTS_HIP(hipSetDevice(device));
+        else before = -1;
+    }
+    ~OnDevice() { if (before >= 0) (void)hipSetDevice(before); }
+};
+
+int compute_units(int device) {
+    static std::atomic<int> known[64];
+    const int k = device & 63;
+    int n = known[k].load();
+    if (n == 0) {
+        PTTS_HIP(hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, device));
+        known[k].store(n);
+    }
+    return n;
+}
+
+}  // namespace
+
+POCKET_TTS_API int ptts_paged_plan(const PttsPagedPlan* plan, int device, void* stream) {
+    if (!plan) { set_error("Invalid parameters"); return -1; }
+    return guarded("paged_plan: ", [&] {
+        ptts::check_paged_plan(*plan);
+        OnDevice on(device);
+        ptts::launch_paged_plan(*plan, static_cast<hipStream_t>(stream));
+        ptts::check_launches("the block-table plan");
+        return 0;
+    });
+}
+
+POCKET_TTS_API int ptts_rotary_frequencies(int rot_dim, double base, int scaling, double factor, double trained, double fast, double slow,
+                                           double* out, float* magnitude) {
+    if (!out || rot_dim < 2 || rot_dim % 2) { set_error("Invalid parameters"); return -1; }
+    return guarded("rotary_frequencies: ", [&] {
+        ptts::rotary_frequencies(rot_dim, base, scaling, factor, trained, fast, slow, out, magnitude);
+        return 0;
+    });
+}
+
+POCKET_TTS_API int ptts_rotary_append(const PttsRotaryAppend* args, int device, void* stream) {
+    if (!args) { set_error("Invalid parameters"); return -1; }
+    return guarded("", [&] {
+        ptts::check_rotary_append(*args);
+        OnDevice on(device);
+        ptts::launch_rotary_append(*args, static_cast<hipStream_t>(stream));
+        ptts::check_launches("the rotary append");
+        return 0;
+    });
+}
+
+POCKET_TTS_API long long ptts_paged_attention_workspace(const PttsPagedAttention* args, int device) {
+    if (!args) { set_error("Invalid parameters"); return -1; }
+    long long n = -1;
+    guarded("", [&] {
+        ptts::check_paged_attention(*args);
+        OnDevice on(device);
+        n = ptts::paged_attention_workspace(*args, compute_units(device));
+        return 0;
+    });
+    return n;
+}
+
+POCKET_TTS_API int ptts_paged_attention(const PttsPagedAttention* args, int device, void* stream) {
+    if (!args) { set_error("Invalid parameters"); return -1; }
+    return guarded("", [&] {
+        ptts::check_paged_attention(*args);
+        OnDevice on(device);
+        ptts::launch_paged_attention(*args, compute_units(device), static_cast<hipStream_t>(stream));
+        ptts::check_launches("the paged attention");
+        return 0;
+    });
+}
 
 // ------------------------------------------------------------------ weights inside an ONNX file (host only)
 

@@ -1,0 +1,43 @@
+// Launch interface of the paged-cache kernels (paged_plan.hip, paged_rotary.hip, paged_attention.hip).  The argument structures
+// are the public ones of pocket_tts_amd.h.  The check_ functions read the structure alone, need no GPU and throw
+// std::runtime_error; the launches take what has passed them, with the device current.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include "pocket_tts/pocket_tts_amd.h"
+
+namespace ptts {
+
+void check_paged_plan(const PttsPagedPlan& p);
+void check_rotary_append(const PttsRotaryAppend& p);
+void check_paged_attention(const PttsPagedAttention& p);
+void launch_paged_plan(const PttsPagedPlan& p, hipStream_t s);
+void launch_rotary_append(const PttsRotaryAppend& a, hipStream_t s);
+long long paged_attention_workspace(const PttsPagedAttention& a, int cus);
+void launch_paged_attention(const PttsPagedAttention& a, int cus, hipStream_t s);
+
+// Host: frequencies in radians per position and the magnitude of the rotated values (pocket_tts_amd.h).
+void rotary_frequencies(int rot_dim, double base, int scaling, double factor, double trained, double fast, double slow, double* out,
+                        float* magnitude);
+
+// The part of the checks that two of them share.
+void check_pages(const PttsPages& p, const char* who);
+
+constexpr int kStatusPage = 1, kStatusRows = 2, kStatusLength = 4;
+
+inline int type_size(int t) { return t == PTTS_TYPE_F32 ? 4 : 2; }
+
+// Quotients of non-negative 31-bit numbers by a number fixed at launch: q = n * m >> s with s = 31 + ceil(log2 d) and
+// m = floor(2^s / d) + 1 < 2^32 (n * (m - 2^s / d) / 2^s < 2^31 / 2^s <= 1 / d, so the quotient is exact).
+struct FastDiv {
+    unsigned m, s, d;
+    static FastDiv of(unsigned d) {
+        unsigned l = 0;
+        while ((1ull << l) < d) ++l;
+        return FastDiv{static_cast<unsigned>((1ull << (31 + l)) / d + 1), 31 + l, d};
+    }
+    __device__ __forceinline__ unsigned div(unsigned n) const { return static_cast<unsigned>((static_cast<unsigned long long>(n) * m) >> s); }
+};
+
+}  // namespace ptts

@@ -15,6 +15,7 @@ PKG = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 LIB_PATH = os.environ.get("POCKET_TTS_LIB") or os.path.join(PKG, "libpocket_tts.so")   # POCKET_TTS_LIB: another build of the library
 
 f32p = np.ctypeslib.ndpointer(dtype=np.float32, flags="C_CONTIGUOUS")
+f64p = np.ctypeslib.ndpointer(dtype=np.float64, flags="C_CONTIGUOUS")
 i64p = np.ctypeslib.ndpointer(dtype=np.int64, flags="C_CONTIGUOUS")
 
 
@@ -56,13 +57,39 @@ EXT_SYMBOLS = [
     "ptts_audio_load_wav", "ptts_audio_save_wav", "ptts_audio_resample", "ptts_audio_normalize",
     "ptts_onnx_open", "ptts_onnx_close", "ptts_onnx_tensor_count", "ptts_onnx_tensor_info", "ptts_onnx_find",
     "ptts_onnx_read_f32", "ptts_onnx_dequantize", "ptts_onnx_node_count", "ptts_onnx_node_info",
+    "ptts_paged_plan", "ptts_rotary_frequencies", "ptts_rotary_append", "ptts_paged_attention_workspace", "ptts_paged_attention",
 ]
 
 _lib = None
+runtime = None   # whose HIP runtime the library is bound to once it is loaded: "system" or "torch"
+
+
+def load_with_torch() -> C.CDLL:
+    """The library bound to the HIP runtime inside the PyTorch wheel, for programs that hand torch tensors to it.
+
+    The wheel carries its own copy of the runtime, and two copies in one process cannot both use the GPU.  This puts the wheel's
+    symbols in front of the system's before the library is opened; it has to be the first load in the process."""
+    global runtime
+    if _lib is None:
+        import torch
+        path = os.path.join(os.path.dirname(torch.__file__), "lib", "libamdhip64.so")
+        if not os.path.exists(path):
+            raise RuntimeError(f"{path} is missing: this PyTorch brings no HIP runtime of its own")
+        C.CDLL(path, mode=C.RTLD_GLOBAL)
+        runtime = "torch"
+        try:
+            return load()
+        except Exception:
+            runtime = None
+            raise
+    if runtime != "torch":
+        raise PttsError("libpocket_tts.so is bound to the system's HIP runtime already: call ptts_lib.load_with_torch() "
+                        "before anything else loads it")
+    return _lib
 
 
 def load() -> C.CDLL:
-    global _lib
+    global _lib, runtime
     if _lib is not None:
         return _lib
     if not os.path.exists(LIB_PATH):
@@ -126,6 +153,12 @@ def load() -> C.CDLL:
     L.ptts_q8_linear_q.restype = ci; L.ptts_q8_linear_q.argtypes = [vp, f32p, ci, ci, vp, f32p, ci, f32p]
     L.ptts_bf16_linear.restype = ci
     L.ptts_bf16_linear.argtypes = [vp, f32p, ci, ci, f32p, ci, vp, vp, vp, ci, ci, f32p]
+    L.ptts_paged_plan.restype = ci; L.ptts_paged_plan.argtypes = [cp, ci, vp]
+    L.ptts_rotary_append.restype = ci; L.ptts_rotary_append.argtypes = [cp, ci, vp]
+    L.ptts_paged_attention.restype = ci; L.ptts_paged_attention.argtypes = [cp, ci, vp]
+    L.ptts_paged_attention_workspace.restype = C.c_longlong; L.ptts_paged_attention_workspace.argtypes = [cp, ci]
+    L.ptts_rotary_frequencies.restype = ci
+    L.ptts_rotary_frequencies.argtypes = [ci, C.c_double, ci, C.c_double, C.c_double, C.c_double, C.c_double, f64p, C.POINTER(C.c_float)]
     L.ptts_weight_bytes.restype = ci; L.ptts_weight_bytes.argtypes = [vp, C.POINTER(C.c_ulonglong)]
     L.ptts_tokenizer_new.restype = vp; L.ptts_tokenizer_new.argtypes = [cp]
     L.ptts_tokenizer_free.restype = None; L.ptts_tokenizer_free.argtypes = [vp]
@@ -136,6 +169,7 @@ def load() -> C.CDLL:
     L.ptts_audio_resample.restype = ci; L.ptts_audio_resample.argtypes = [f32p, ci, ci, ci, f32p, ci]
     L.ptts_audio_normalize.restype = ci; L.ptts_audio_normalize.argtypes = [f32p, ci, f32p]
     _lib = L
+    runtime = runtime or "system"
     return L
 
 
