@@ -1,8 +1,25 @@
 // Attention of every request's new rows over its pages (pocket_tts_amd.h, ptts_paged_attention).
+//
+// The G query heads of a key head share its keys, so the rows of one request and one key head are packed: packed row m is new
+// row m / G under head m % G.  Three kernels work on tiles of packed rows:
+//
+//   chunk   128 packed rows, four waves of 32; key blocks of 64 go through LDS and are read by all four waves
+//   few     16 packed rows; four waves walk different keys straight from memory and join at the end (single tokens: bound by
+//           the one read of the keys and values)
+//   merge   joins the parts of rows whose keys were cut into splits
+//
+// All products are formed transposed, S^T = K Q^T and O^T = V^T P^T, so that a lane keeps one query for the whole kernel (its
+// running maximum and sum are scalars of the lane) and the weights leave the first product in the layout the second one takes
+// them in.  Softmax statistics and both sums are float32; the weights are rounded once, to the rows' type, because the matrix
+// instructions take both operands in one type (at most half a step of the type on each weight; float rows keep float weights).
+//
+// The running maximum is a reference that lags: sums are rescaled only when a score passes it by 2^8, which leaves every weight
+// below 2^8, far inside float16, and saves most rescales.
 #include <algorithm>
 #include <cmath>
 #include <stdexcept>
 #include <string>
+#include <type_traits>
 
 #include "paged.h"
 
@@ -10,90 +27,780 @@ namespace ptts {
 
 namespace {
 
-struct AttnArgs {
-    PttsPagedAttention p;
-    FastDiv page;
-    int group;            // query heads per key head
-    float scale2;         // scale * log2(e)
+constexpr int kChunkRows = 128, kChunkKeys = 64;   // chunk kernel: packed rows of a workgroup, keys of a block
+constexpr int kFewRows = 16;                       // few kernel: packed rows of a workgroup
+constexpr float kLn2 = 0.69314718055994531f, kLag = 8.0f;
+
+// How a call is cut: which kernels run, over how many tiles, into how many splits of the keys.
+struct Cut {
+    bool chunk = false, few = false;
+    int small = 0;              // both kernels run: requests of at most this many packed rows go to the few kernel
+    int few_direct = 0;         // ... which then gives each request this many tiles; 0: tiles are found by search
+    int few_keys = 0;           // keys of one step of a workgroup of the few kernel
+    long long chunk_tiles = 0, few_tiles = 0;
+    int chunk_splits = 1, few_splits = 1;
+    int chunk_least = 1, few_least = 1;   // fewest key blocks of a split
+    long long bytes = 0;
 };
 
-// The request that owns a row, or -1: the last i with cu_rows[i] <= row, found 64 requests at a time.
-__device__ __forceinline__ int request_of_row(const PttsPagedAttention& p, int row) {
-    const int lane = threadIdx.x & 63;
-    int lo = 0, span = p.requests;
-    while (span > 1) {
-        const int step = (span + 63) >> 6, i = lo + lane * step;
-        const int hits = __popcll(__ballot(lane * step < span && p.cu_rows[i] <= row));
-        if (hits == 0) return -1;
-        const int left = span - (hits - 1) * step;
-        lo += (hits - 1) * step;
-        span = left < step ? left : step;
-    }
-    return p.cu_rows[lo] <= row && row < p.cu_rows[lo + 1] ? lo : -1;
+struct AttnArgs {
+    PttsPagedAttention p;
+    FastDiv page, group;
+    float scale2;               // scale * log2(e)
+    long long tiles;            // of the kernel that is launched
+    int splits, least, small, direct;
+    int merge_few, merge_chunk; // splits of the two kernels' rows (merge)
+    float* part;                // [split][row][head][dim], then [split][row][head] of log2 sum exp2
+    float* part_lse;
+};
+
+typedef __attribute__((ext_vector_type(4))) float f32x4;
+typedef __attribute__((ext_vector_type(16))) float f32x16;
+typedef __attribute__((ext_vector_type(4))) short s16x4;
+template <typename T> using x8 = T __attribute__((ext_vector_type(8)));
+template <typename T> using x4 = T __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ f32x16 mma32(x8<__bf16> a, x8<__bf16> b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x16 mma32(x8<_Float16> a, x8<_Float16> b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x4 mma16(x8<__bf16> a, x8<__bf16> b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x4 mma16(x8<_Float16> a, x8<_Float16> b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+
+// Both halves of the wave (all four rows of 16 lanes) combined, result in every lane.
+__device__ __forceinline__ float max_half(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float sum_half(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float max_rows(float x) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return max_half(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+}
+__device__ __forceinline__ float sum_rows(float x) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return sum_half(__uint_as_float(r[0]) + __uint_as_float(r[1]));
 }
 
-// Plain form: one wave per (row, head), 64 keys at a time.  A lane forms the whole product of its own key with the query; the
-// weighted sum walks the visible keys with the lanes on the head's values.
-template <typename T, typename C>
-__global__ __launch_bounds__(256) void attention_rows_kernel(AttnArgs a) {
+// A tile of packed rows: the request that owns it and what its rows see.
+struct Tile {
+    int i, row0, n, len, pos0;      // request, its first row, row count, length, position of its first row
+    int m0, m1;                     // packed rows m0 .. m1 - 1 of the request
+    int p0, p1;                     // positions of the first and the last row of the tile
+    int low;                        // first key of the window of row m0 (the lowest of the tile)
+    int bad;
+};
+
+// Tile numbers of request i begin at cu_rows[i] * G / BM + i: its ceil(n G / BM) tiles end before those of the next request
+// begin, so a tile finds its request without prefix sums, 64 requests at a time, and a few numbers stay unused.
+__device__ __forceinline__ bool find_tile(const AttnArgs& a, long long tile, int rows_per_tile, Tile& t) {
     const PttsPagedAttention& p = a.p;
-    const int lane = threadIdx.x & 63;
-    const long long unit = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int row = (int)(unit / p.q_heads), head = (int)(unit % p.q_heads);
-    if (row >= p.rows) return;
-    const int i = request_of_row(p, row);
-    if (i < 0) return;
-    const int r0 = p.cu_rows[i], r1 = p.cu_rows[i + 1];
-    int len = p.kv_len[i], bad = 0;
-    const long long cap = (long long)p.table_width * p.pages.page_size;
-    if (r0 < 0 || r1 > p.rows) bad |= kStatusRows;
-    if (len < 0) { len = 0; bad |= kStatusLength; }
-    if (len > cap) { len = (int)cap; bad |= kStatusLength; }
-    const int pos = len - (r1 - row);
-    const int dim = p.pages.head_dim, kvh = head / a.group;
-    const T* q = (const T*)p.q + (long long)row * p.q_row_stride + (long long)head * p.q_head_stride;
-    const int* table = p.block_table + (long long)i * p.table_stride;
-    float m = -INFINITY, l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-    int lo = p.window > 0 && pos - p.window + 1 > 0 ? pos - p.window + 1 : 0;
-    for (int k0 = 0; k0 <= pos; k0 += 64) {
-        if (p.window > 0 && k0 >= p.sinks && k0 + 63 < lo) { k0 = lo / 64 * 64; }
-        const int key = k0 + lane;
-        bool see = key <= pos && (key >= lo || key < p.sinks);
-        long long at = -1;
-        if (see) {
-            const int pg = (int)a.page.div(key), id = table[pg];
-            if (id < 0 || id >= p.pages.pages) bad |= kStatusPage;
-            else at = (long long)id * p.pages.page_stride + (long long)(key - pg * p.pages.page_size) * p.pages.row_stride + (long long)kvh * p.pages.head_stride;
+    const int lane = threadIdx.x & 63, G = a.group.d;
+    int sub;
+    if (a.direct) {
+        t.i = (int)(tile / a.direct);
+        sub = (int)(tile - (long long)t.i * a.direct);
+    } else {
+        int lo = 0, span = p.requests;
+        while (span > 1) {
+            const int step = (span + 63) >> 6, i = lo + lane * step;
+            const bool hit = lane * step < span && (long long)p.cu_rows[i] * G / rows_per_tile + i <= tile;
+            const int hits = __popcll(__ballot(hit));
+            if (hits == 0) return false;
+            const int left = span - (hits - 1) * step;
+            lo += (hits - 1) * step;
+            span = left < step ? left : step;
         }
-        float s = 0.f;
-        if (at >= 0) for (int d = 0; d < dim; ++d) s += (float)q[d] * (float)((const C*)p.pages.k)[at + d];
-        s = see ? s * a.scale2 : -INFINITY;
-        float top = s;
-        for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
-        const float mn = fmaxf(m, top);
-        if (mn == -INFINITY) continue;
-        const float w = see ? exp2f(s - mn) : 0.f, fade = exp2f(m - mn);
-        float ws = w;
-        for (int o = 32; o > 0; o >>= 1) ws += __shfl_xor(ws, o, 64);
-        l = l * fade + ws;
-        m = mn;
-        for (int c = 0; c < 4; ++c) acc[c] *= fade;
-        unsigned long long left = __ballot(at >= 0);
-        while (left) {
-            const int j = __builtin_ctzll(left);
-            left &= left - 1;
-            const float wj = __shfl(w, j, 64);
-            const long long aj = __shfl(at, j, 64);
-            for (int c = 0; c < 4; ++c)
-                if (lane + 64 * c < dim) acc[c] += wj * (float)((const C*)p.pages.v)[aj + lane + 64 * c];
+        t.i = __builtin_amdgcn_readfirstlane(lo);
+        const long long first = (long long)p.cu_rows[t.i] * G / rows_per_tile + t.i;
+        if (tile < first || tile - first > 0x7fffffff) return false;
+        sub = (int)(tile - first);
+    }
+    t.row0 = p.cu_rows[t.i];
+    const int end = p.cu_rows[t.i + 1];
+    t.bad = 0;
+    t.n = end - t.row0;
+    if (t.row0 < 0 || end > p.rows || end < t.row0) {
+        if (p.status && threadIdx.x == 0) atomicOr(p.status, kStatusRows);
+        return false;
+    }
+    t.len = p.kv_len[t.i];
+    const int cap = p.table_width * p.pages.page_size;
+    if (t.len < 0) { t.len = 0; t.bad = kStatusLength; }
+    if (t.len > cap) { t.len = cap; t.bad = kStatusLength; }
+    const long long packed = (long long)t.n * G, from = (long long)sub * rows_per_tile;
+    if (from >= packed) return false;
+    t.m0 = (int)from;
+    t.m1 = (int)(packed - from < rows_per_tile ? packed : from + rows_per_tile);
+    t.pos0 = t.len - t.n;
+    t.p0 = t.pos0 + (int)a.group.div(t.m0);
+    t.p1 = t.pos0 + (int)a.group.div(t.m1 - 1);
+    t.low = p.window > 0 && t.p0 - p.window + 1 > 0 ? t.p0 - p.window + 1 : 0;
+    return true;
+}
+
+// The key blocks that a tile has to look at: those of the sinks, then those from the window's first key to the last row's own.
+struct Blocks {
+    int sink, start, count;
+    __device__ __forceinline__ Blocks(const Tile& t, int sinks, int keys) {
+        sink = 0;
+        start = t.low / keys;
+        if (t.low > 0 && sinks > 0) sink = ((sinks < t.low ? sinks : t.low) + keys - 1) / keys;
+        if (start < sink) start = sink;
+        count = t.p1 < 0 ? 0 : sink + (t.p1 / keys - start + 1 > 0 ? t.p1 / keys - start + 1 : 0);
+    }
+    __device__ __forceinline__ int block(int u) const { return u < sink ? u : start + u - sink; }
+};
+
+__device__ __forceinline__ bool seen(const PttsPagedAttention& p, int key, int pos) {
+    return key <= pos && (p.window <= 0 || key > pos - p.window || key < p.sinks);
+}
+// whether rows at positions p0 .. p1 all see the keys k0 .. k1 / whether none of them sees any
+__device__ __forceinline__ bool all_seen(const PttsPagedAttention& p, int k0, int k1, int p0, int p1) {
+    return k1 <= p0 && (p.window <= 0 || k0 > p1 - p.window || k1 < p.sinks);
+}
+__device__ __forceinline__ bool none_seen(const PttsPagedAttention& p, int k0, int k1, int p0, int p1) {
+    return k0 > p1 || (p.window > 0 && k1 <= p0 - p.window && k0 >= p.sinks);
+}
+
+// Element offset of a key's row under one key head, -1 where no row of the tile sees it (then it reads as zeros, so that nothing
+// stale reaches a product) or where its page id is not one.
+__device__ __forceinline__ int page_of(const AttnArgs& a, const Tile& t, const int* table, int key) {
+    if (key > t.p1 || (key < t.low && key >= a.p.sinks)) return -1;
+    const int id = table[a.page.div(key)];
+    return id >= 0 && id < a.p.pages.pages ? id : -2;
+}
+__device__ __forceinline__ long long row_at(const AttnArgs& a, int id, int key, int kvh) {
+    const PttsPages& g = a.p.pages;
+    return id < 0 ? -1 : (long long)id * g.page_stride + (long long)(key - (int)a.page.div(key) * g.page_size) * g.row_stride + (long long)kvh * g.head_stride;
+}
+
+// Values that are NaN or infinite and stand at keys which only some rows of a tile see must not meet the other rows' zero weights.
+// Such a block is rare (it needs a block at the border of what is seen, and a value that is not finite): its values are split into
+// finite ones, which the product takes, and 0/1 marks of NaN and of the infinities, whose products with the 0/1 pattern of seen
+// keys say which sums they reach.
+template <typename T> __device__ __forceinline__ bool not_finite2(unsigned w) {
+    constexpr unsigned e = std::is_same<T, __bf16>::value ? 0x7f80u : 0x7c00u;
+    return (w & e) == e || ((w >> 16) & e) == e;
+}
+template <typename T> __device__ __forceinline__ bool not_finite(uint4 w) {
+    return not_finite2<T>(w.x) || not_finite2<T>(w.y) || not_finite2<T>(w.z) || not_finite2<T>(w.w);
+}
+// kind 0: the finite values, zero elsewhere; 1, 2, 3: ones where a value is NaN, positive, negative infinity
+template <typename T> __device__ __forceinline__ x8<T> marked(x8<T> v, int kind) {
+    x8<T> y;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const float f = (float)v[j], mark = (kind == 1 ? f != f : kind == 2 ? f == INFINITY : f == -INFINITY) ? 1.f : 0.f;
+        y[j] = (T)(kind == 0 ? (fabsf(f) < INFINITY ? f : 0.f) : mark);
+    }
+    return y;
+}
+__device__ __forceinline__ float with_mark(float sum, float hits, int kind) {
+    return hits > 0.f ? kind == 1 ? NAN : kind == 2 ? sum + INFINITY : sum - INFINITY : sum;
+}
+
+// exp2 of what is at most kLag; denormals flush to zero
+__device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// ------------------------------------------------------------------ chunk
+
+// LDS holds a block's 64 rows of DH values without padding.  16-byte unit c of row r lies at unit c ^ swizzle(r), which spreads the
+// reads of one instruction over all banks: rows 0 .. 15 at one unit for the keys (16 bytes a lane), eight rows of four units each
+// for the transposed reads of the values (8 bytes a lane).
+template <int DH> __device__ __forceinline__ int key_swizzle(int row) { return DH >= 128 ? row & 15 : (row >> 1) & 7; }
+template <int DH> __device__ __forceinline__ int value_swizzle(int row) { return DH >= 128 ? (row & 3) << 2 : ((row >> 1) & 1) << 2; }
+
+template <typename T, int DH>
+__global__ __launch_bounds__(256, DH == 256 ? 1 : 2) void attention_chunk_kernel(AttnArgs a) {
+    constexpr int kUnits = DH / 8, kPassRows = 256 / kUnits, kPasses = kChunkKeys / kPassRows, KS = DH / 16, NT = DH / 32;
+    __shared__ __attribute__((aligned(16))) T Ks[kChunkKeys * DH];
+    __shared__ __attribute__((aligned(16))) T Vs[kChunkKeys * DH];
+    const PttsPagedAttention& p = a.p;
+    const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, h = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);   // matrix instructions ignore the lane mask: every branch around one is scalar
+    // key heads first (neighbouring workgroups go to different dies, so a die's cache sees few heads), and the tiles that see
+    // most keys first
+    const int kvh = blockIdx.x % p.pages.kv_heads;
+    const unsigned rest = blockIdx.x / p.pages.kv_heads;
+    const int split = rest % a.splits;
+    Tile t;
+    if (!find_tile(a, a.tiles - 1 - rest / a.splits, kChunkRows, t)) return;
+    const int G = a.group.d, dim = p.pages.head_dim;
+    if ((long long)t.n * G <= a.small) return;
+    const Blocks list(t, p.sinks, kChunkKeys);
+    const int per = max(a.least, (list.count + a.splits - 1) / a.splits);
+    const int u0 = split * per, u1 = min(list.count, u0 + per);
+
+    // this lane's query, and the positions of this wave's rows
+    const int mw = t.m0 + wave * 32, m = min(mw + col, t.m1 - 1), tok = a.group.div(m), head = kvh * G + m - tok * G;
+    const bool live = mw + col < t.m1;
+    const int pos = t.pos0 + tok, row = t.row0 + tok;
+    const int pw0 = t.pos0 + (int)a.group.div(min(mw, t.m1 - 1)), pw1 = t.pos0 + (int)a.group.div(min(mw + 31, t.m1 - 1));
+    const bool idle = mw >= t.m1;
+    x8<T> qf[KS];
+    {
+        const T* q = (const T*)p.q + (long long)row * p.q_row_stride + (long long)head * p.q_head_stride + 8 * h;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            const x8<T> zero = {};
+            qf[ks] = 16 * ks + 8 * h < dim ? *(const x8<T>*)(q + 16 * ks) : zero;
+        }
+    }
+
+    const int* table = p.block_table + (long long)t.i * p.table_stride;
+    const int unit = tid % kUnits, sr = tid / kUnits;
+    const bool unit_live = unit * 8 < dim;
+    int ids[kPasses];
+    uint4 kreg[kPasses], vreg[kPasses];
+    int bad = t.bad;
+    auto look_up = [&](int u) {
+        const int k0 = list.block(u) * kChunkKeys;
+#pragma unroll
+        for (int i = 0; i < kPasses; ++i) ids[i] = page_of(a, t, table, k0 + sr + kPassRows * i);
+    };
+    auto load = [&](int u) {
+        const int k0 = list.block(u) * kChunkKeys;
+#pragma unroll
+        for (int i = 0; i < kPasses; ++i) {
+            if (ids[i] == -2) bad |= kStatusPage;
+            const long long at = row_at(a, ids[i], k0 + sr + kPassRows * i, kvh);
+            kreg[i] = vreg[i] = make_uint4(0, 0, 0, 0);
+            if (at >= 0 && unit_live) {
+                kreg[i] = *(const uint4*)((const T*)p.pages.k + at + unit * 8);
+                vreg[i] = *(const uint4*)((const T*)p.pages.v + at + unit * 8);
+            }
+        }
+    };
+
+    f32x16 o[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[n][r] = 0.f;
+    float top = -INFINITY, sum = 0.f;      // reference of the exponents in log2 units, this lane's part of the sum
+
+    const int ky = key_swizzle<DH>(col) ^ h;
+    const int vrow = 4 * h + ((lane & 15) >> 2);
+    const T* vbase = Vs + vrow * DH + 4 * (lane & 1);
+    const int vunit = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), vx = value_swizzle<DH>(vrow);
+    auto value = [&](int n, int s) {        // V^T of 32 head values from 32 n and keys 16 s ..: keys 4 h + 0..3 and 8 + 4 h + 0..3
+        const T* at = vbase + 16 * s * DH + ((4 * n + vunit) ^ vx) * 8;
+        union { s16x4 w[2]; x8<T> v; } u;
+        u.w[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at);
+        u.w[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(at + 8 * DH));
+        return u.v;
+    };
+
+    if (u0 < u1) {
+        look_up(u0);
+        load(u0);
+        if (u0 + 1 < u1) look_up(u0 + 1);
+    }
+    for (int u = u0; u < u1; ++u) {
+        const int k0 = list.block(u) * kChunkKeys, k1 = k0 + kChunkKeys - 1;
+        bool odd = false;                   // values that are not finite in a block that not every row sees whole
+        if (!all_seen(p, k0, k1, t.p0, t.p1)) {
+#pragma unroll
+            for (int i = 0; i < kPasses; ++i) odd |= not_finite<T>(vreg[i]);
+            odd = __builtin_amdgcn_readfirstlane(__syncthreads_or(odd));
+        } else {
+            __syncthreads();                // the previous block is consumed
+        }
+#pragma unroll
+        for (int i = 0; i < kPasses; ++i) {
+            const int r = sr + kPassRows * i;
+            *(uint4*)(Ks + r * DH + (unit ^ key_swizzle<DH>(r)) * 8) = kreg[i];
+            *(uint4*)(Vs + r * DH + (unit ^ value_swizzle<DH>(r)) * 8) = vreg[i];
+        }
+        __syncthreads();
+        if (u + 1 < u1) {
+            load(u + 1);
+            if (u + 2 < u1) look_up(u + 2);
+        }
+        if (idle || none_seen(p, k0, k1, pw0, pw1)) continue;
+
+        f32x16 s[2];
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[b][r] = 0.f;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks)
+                s[b] = mma32(*(const x8<T>*)(Ks + (32 * b + col) * DH + ((2 * ks) ^ ky) * 8), qf[ks], s[b]);
+        }
+        // lane: query col; s[b][r] belongs to key k0 + 32 b + 8 (r / 4) + 4 h + r % 4
+        unsigned mask = ~0u;
+        if (!all_seen(p, k0, k1, pw0, pw1)) {
+            mask = 0;
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const bool ok = seen(p, k0 + 32 * b + 8 * (r >> 2) + 4 * h + (r & 3), pos);
+                    mask |= ok ? 1u << (16 * b + r) : 0u;
+                    s[b][r] = ok ? s[b][r] : -INFINITY;
+                }
+        }
+        float best = s[0][0];
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) best = fmaxf(best, s[b][r]);
+        best = max_half(best) * a.scale2;
+        if (__any(best > top + kLag)) {
+            const float next = fmaxf(top, best), fade = top == -INFINITY ? 0.f : exp2_of(top - next);
+            top = next;
+            sum *= fade;
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[n][r] *= fade;
+        }
+        const float base = top == -INFINITY ? 0.f : top;
+        x8<T> w[4];
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const float e = exp2_of(__builtin_fmaf(s[b][r], a.scale2, -base));
+                sum += e;
+                w[2 * b + (r >> 3)][r & 7] = (T)e;
+            }
+        if (!odd) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) o[n] = mma32(value(n, k), w[k], o[n]);
+        } else {
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) o[n] = mma32(marked(value(n, k), 0), w[k], o[n]);
+            x8<T> see[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) see[k][j] = (T)((mask >> (8 * k + j)) & 1 ? 1.f : 0.f);
+#pragma unroll 1
+            for (int kind = 1; kind < 4; ++kind)
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    f32x16 c;
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) c[r] = 0.f;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) c = mma32(marked(value(n, k), kind), see[k], c);
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) o[n][r] = with_mark(o[n][r], c[r], kind);
+                }
+        }
+    }
+
+    if (bad && p.status) atomicOr(p.status, bad);
+    sum = sum_half(sum);
+    if (!live) return;
+    const float inv = sum == 0.f ? 0.f : 1.0f / sum, lse2 = sum == 0.f ? -INFINITY : top + __log2f(sum);
+    if (a.splits == 1) {
+        T* out = (T*)p.out + (long long)row * p.out_row_stride + (long long)head * p.out_head_stride + 4 * h;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if (32 * n + 8 * q < dim) {
+                    x4<T> v;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) v[r] = (T)(sum == 0.f ? 0.f : o[n][4 * q + r] * inv);
+                    *(x4<T>*)(out + 32 * n + 8 * q) = v;
+                }
+        if (p.lse && h == 0) p.lse[(long long)row * p.lse_row_stride + head] = lse2 * kLn2;
+    } else {
+        const long long at = ((long long)split * p.rows + row) * p.q_heads + head;
+        float* part = a.part + at * dim + 4 * h;
+        if (sum != 0.f)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    if (32 * n + 8 * q < dim)
+                        *(f32x4*)(part + 32 * n + 8 * q) = f32x4{o[n][4 * q] * inv, o[n][4 * q + 1] * inv, o[n][4 * q + 2] * inv, o[n][4 * q + 3] * inv};
+        if (h == 0) a.part_lse[at] = lse2;
+    }
+}
+
+// ------------------------------------------------------------------ few
+
+// Fragments of one step of a wave, straight from memory: NA blocks of 16 keys.  Keys: lane (row lane % 16, quarter g = lane / 16) reads
+// the units g of its row.  Values: the lane reads head values CPL m .. CPL m + CPL - 1 (m = lane % 16) of the rows 4 g + r, so that
+// column t of every lane forms the operand of output tile t; the output's order is then CPL * (its row) + t.
+template <typename T, typename C, int DH> struct Step {
+    static constexpr bool kFloat = std::is_same<T, float>::value;
+    static constexpr int NA = kFloat ? 1 : 2, CPL = DH / 16, KS = kFloat ? DH / 16 : DH / 32, KW = kFloat ? 4 : 8;
+    static constexpr int VW = CPL < 8 ? CPL : 8, VN = CPL / VW;     // values of one access, accesses of a row
+    typedef C kvec __attribute__((ext_vector_type(KW)));
+    typedef C vvec __attribute__((ext_vector_type(VW)));
+    kvec k[NA][KS];
+    vvec v[4 * NA][VN];
+};
+
+template <typename T, typename C, int DH>
+__global__ __launch_bounds__(256, DH == 256 ? 1 : 2) void attention_few_kernel(AttnArgs a) {
+    using S = Step<T, C, DH>;
+    constexpr int NA = S::NA, CPL = S::CPL, KS = S::KS, KW = S::KW, VW = S::VW, VN = S::VN, kWaveKeys = 16 * NA, kKeys = 4 * kWaveKeys;
+    constexpr bool kFloat = S::kFloat;
+    __shared__ float joined[4][kFewRows][DH + 4];      // +4: the waves' columns of one row do not meet in one bank
+    __shared__ float tops[4][kFewRows], sums[4][kFewRows];
+    const PttsPagedAttention& p = a.p;
+    const int tid = threadIdx.x, lane = tid & 63, li = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);   // matrix instructions ignore the lane mask: every branch around one is scalar
+    const int kvh = blockIdx.x % p.pages.kv_heads;
+    const unsigned rest = blockIdx.x / p.pages.kv_heads;
+    const int split = rest % a.splits;
+    Tile t;
+    if (!find_tile(a, rest / a.splits, kFewRows, t)) return;
+    const int G = a.group.d, dim = p.pages.head_dim;
+    if (a.small > 0 && (long long)t.n * G > a.small) return;
+    const Blocks list(t, p.sinks, kKeys);
+    const int per = max(a.least, (list.count + a.splits - 1) / a.splits);
+    const int u0 = split * per, u1 = min(list.count, u0 + per);
+
+    const int m = min(t.m0 + li, t.m1 - 1), tok = a.group.div(m), head = kvh * G + m - tok * G, row = t.row0 + tok, pos = t.pos0 + tok;
+    T qf[KS][KW];
+    {
+        const T* q = (const T*)p.q + (long long)row * p.q_row_stride + (long long)head * p.q_head_stride + KW * g;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+            for (int j = 0; j < KW; ++j) qf[ks][j] = 4 * KW * ks + KW * g < dim ? q[4 * KW * ks + j] : (T)0.f;
+    }
+
+    const int* table = p.block_table + (long long)t.i * p.table_stride;
+    int bad = t.bad, ids[NA];
+    auto look_up = [&](int u) {
+        const int k0 = list.block(u) * kKeys + wave * kWaveKeys;
+#pragma unroll
+        for (int b = 0; b < NA; ++b) ids[b] = page_of(a, t, table, k0 + 16 * b + li);
+    };
+    auto load = [&](int u, S& x) {
+        const int k0 = list.block(u) * kKeys + wave * kWaveKeys;
+#pragma unroll
+        for (int b = 0; b < NA; ++b) {
+            if (ids[b] == -2) bad |= kStatusPage;
+            const long long at = row_at(a, ids[b], k0 + 16 * b + li, kvh);
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                const typename S::kvec zero = {};
+                const int d = 4 * KW * ks + KW * g;
+                x.k[b][ks] = at >= 0 && d < dim ? *(const typename S::kvec*)((const C*)p.pages.k + at + d) : zero;
+            }
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const long long from = __shfl(at, 4 * g + r, 64);
+#pragma unroll
+                for (int n = 0; n < VN; ++n) {
+                    const typename S::vvec zero = {};
+                    const int d = CPL * li + VW * n;
+                    x.v[4 * b + r][n] = from >= 0 && d < dim ? *(const typename S::vvec*)((const C*)p.pages.v + from + d) : zero;
+                }
+            }
+        }
+    };
+
+    f32x4 o[CPL];
+#pragma unroll
+    for (int n = 0; n < CPL; ++n) o[n] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float top = -INFINITY, sum = 0.f;
+
+    auto work = [&](int u, const S& x) {
+        const int k0 = list.block(u) * kKeys + wave * kWaveKeys, k1 = k0 + kWaveKeys - 1;
+        if (none_seen(p, k0, k1, t.p0, t.p1)) return;
+        f32x4 s[NA];
+#pragma unroll
+        for (int b = 0; b < NA; ++b) {
+            s[b] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                if constexpr (kFloat) {
+#pragma unroll
+                    for (int j = 0; j < KW; ++j) s[b] = __builtin_amdgcn_mfma_f32_16x16x4f32((float)x.k[b][ks][j], qf[ks][j], s[b], 0, 0, 0);
+                } else {
+                    x8<T> q;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) q[j] = qf[ks][j];
+                    s[b] = mma16(x.k[b][ks], q, s[b]);
+                }
+            }
+        }
+        // lane: query li; s[b][r] belongs to key k0 + 16 b + 4 g + r
+        const bool whole = all_seen(p, k0, k1, t.p0, t.p1);
+        unsigned mask = ~0u;
+        if (!whole) {
+            mask = 0;
+#pragma unroll
+            for (int b = 0; b < NA; ++b)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const bool ok = seen(p, k0 + 16 * b + 4 * g + r, pos);
+                    mask |= ok ? 1u << (4 * b + r) : 0u;
+                    s[b][r] = ok ? s[b][r] : -INFINITY;
+                }
+        }
+        float best = s[0][0];
+#pragma unroll
+        for (int b = 0; b < NA; ++b)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) best = fmaxf(best, s[b][r]);
+        best = max_rows(best) * a.scale2;
+        if (__any(best > top + kLag)) {
+            const float next = fmaxf(top, best), fade = top == -INFINITY ? 0.f : exp2_of(top - next);
+            top = next;
+            sum *= fade;
+#pragma unroll
+            for (int n = 0; n < CPL; ++n) o[n] *= fade;
+        }
+        const float base = top == -INFINITY ? 0.f : top;
+        float e[4 * NA];
+#pragma unroll
+        for (int b = 0; b < NA; ++b)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                e[4 * b + r] = exp2_of(__builtin_fmaf(s[b][r], a.scale2, -base));
+                sum += e[4 * b + r];
+            }
+        // values that are not finite at keys that not every row of the tile sees
+        bool odd = false;
+        if (!whole && t.p0 != t.p1) {
+#pragma unroll
+            for (int r = 0; r < 4 * NA; ++r)
+#pragma unroll
+                for (int n = 0; n < VN; ++n)
+#pragma unroll
+                    for (int j = 0; j < VW; ++j) odd |= !(fabsf((float)x.v[r][n][j]) < INFINITY);
+            odd = __builtin_amdgcn_readfirstlane(__any(odd));
+        }
+        if constexpr (kFloat) {
+#pragma unroll
+            for (int n = 0; n < CPL; ++n) {
+                f32x4 cn = {0.f, 0.f, 0.f, 0.f}, cu = cn, cd = cn;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    float v = (float)x.v[r][n / VW][n % VW];
+                    if (odd) {
+                        const float see = (mask >> r) & 1 ? 1.f : 0.f;
+                        cn = __builtin_amdgcn_mfma_f32_16x16x4f32(v != v ? 1.f : 0.f, see, cn, 0, 0, 0);
+                        cu = __builtin_amdgcn_mfma_f32_16x16x4f32(v == INFINITY ? 1.f : 0.f, see, cu, 0, 0, 0);
+                        cd = __builtin_amdgcn_mfma_f32_16x16x4f32(v == -INFINITY ? 1.f : 0.f, see, cd, 0, 0, 0);
+                        if (!(fabsf(v) < INFINITY)) v = 0.f;
+                    }
+                    o[n] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, e[r], o[n], 0, 0, 0);
+                }
+                if (odd)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) o[n][r] = with_mark(with_mark(with_mark(o[n][r], cn[r], 1), cu[r], 2), cd[r], 3);
+            }
+        } else {
+            x8<T> w, see;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) { w[j] = (T)e[j]; see[j] = (T)((mask >> j) & 1 ? 1.f : 0.f); }
+#pragma unroll
+            for (int n = 0; n < CPL; ++n) {
+                // column n of the eight rows: halves of their registers put together in pairs
+                union { unsigned d[4]; x8<T> v; } u;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    union { typename S::vvec v; unsigned d[VW / 2]; } lo, hi;
+                    lo.v = x.v[2 * j][n / VW];
+                    hi.v = x.v[2 * j + 1][n / VW];
+                    u.d[j] = __builtin_amdgcn_perm(hi.d[n % VW / 2], lo.d[n % VW / 2], n & 1 ? 0x07060302u : 0x05040100u);
+                }
+                if (!odd) {
+                    o[n] = mma16(u.v, w, o[n]);
+                } else {
+                    o[n] = mma16(marked(u.v, 0), w, o[n]);
+#pragma unroll 1
+                    for (int kind = 1; kind < 4; ++kind) {
+                        const f32x4 c = mma16(marked(u.v, kind), see, f32x4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) o[n][r] = with_mark(o[n][r], c[r], kind);
+                    }
+                }
+            }
+        }
+    };
+
+    S one, two;
+    if (u0 < u1) {
+        look_up(u0);
+        load(u0, one);
+        if (u0 + 1 < u1) look_up(u0 + 1);
+    }
+    for (int u = u0; u < u1; u += 2) {
+        if (u + 1 < u1) {
+            load(u + 1, two);
+            if (u + 2 < u1) look_up(u + 2);
+        }
+        work(u, one);
+        if (u + 1 < u1) {
+            if (u + 2 < u1) {
+                load(u + 2, one);
+                if (u + 3 < u1) look_up(u + 3);
+            }
+            work(u + 1, two);
         }
     }
     if (bad && p.status) atomicOr(p.status, bad);
-    T* out = (T*)p.out + (long long)row * p.out_row_stride + (long long)head * p.out_head_stride;
-    const float inv = l == 0.f ? 0.f : 1.0f / l;
-    for (int c = 0; c < 4; ++c)
-        if (lane + 64 * c < dim) out[lane + 64 * c] = (T)(l == 0.f ? 0.f : acc[c] * inv);
-    if (p.lse && lane == 0) p.lse[(long long)row * p.lse_row_stride + head] = l == 0.f ? -INFINITY : m * 0.69314718055994531f + logf(l);
+
+    // join the four waves: lane holds query li, head values CPL (4 g + r) + n
+    sum = sum_rows(sum);
+    if (g == 0) { tops[wave][li] = top; sums[wave][li] = sum; }
+    __syncthreads();
+    float all = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) all = fmaxf(all, tops[w][li]);
+    const float mine = top == -INFINITY ? 0.f : exp2_of(top - all);
+    const int n_live = t.m1 - t.m0;
+    if (li < n_live) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int n = 0; n < CPL; n += 4)
+                *(f32x4*)&joined[wave][li][CPL * (4 * g + r) + n] = f32x4{o[n][r], o[n + 1][r], o[n + 2][r], o[n + 3][r]} * mine;
+    }
+    __syncthreads();
+    const int quads = dim / 4;
+    for (int x = tid; x < n_live * quads; x += 256) {
+        const int q = x / quads, d = 4 * (x - q * quads);
+        float big = -INFINITY, total = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) big = fmaxf(big, tops[w][q]);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) total += tops[w][q] == -INFINITY ? 0.f : sums[w][q] * exp2_of(tops[w][q] - big);
+        f32x4 v = *(f32x4*)&joined[0][q][d];
+#pragma unroll
+        for (int w = 1; w < 4; ++w) v += *(f32x4*)&joined[w][q][d];
+        const float inv = total == 0.f ? 0.f : 1.0f / total, lse2 = total == 0.f ? -INFINITY : big + __log2f(total);
+        const int mq = t.m0 + q, tq = a.group.div(mq), hq = kvh * G + mq - tq * G;
+        const long long rq = t.row0 + tq;
+        if (a.splits == 1) {
+            x4<T> w;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) w[r] = (T)(total == 0.f ? 0.f : v[r] * inv);
+            *(x4<T>*)((T*)p.out + rq * p.out_row_stride + (long long)hq * p.out_head_stride + d) = w;
+            if (p.lse && d == 0) p.lse[rq * p.lse_row_stride + hq] = lse2 * kLn2;
+        } else {
+            const long long at = ((long long)split * p.rows + rq) * p.q_heads + hq;
+            if (total != 0.f) *(f32x4*)(a.part + at * dim + d) = v * inv;
+            if (d == 0) a.part_lse[at] = lse2;
+        }
+    }
+}
+
+// ------------------------------------------------------------------ merge
+
+// One wave per (row, head): out = sum over splits of exp2(lse_s - lse) part_s.
+template <typename T>
+__global__ __launch_bounds__(256) void attention_merge_kernel(AttnArgs a) {
+    const PttsPagedAttention& p = a.p;
+    const int lane = threadIdx.x & 63;
+    const long long unit = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int row = (int)(unit / p.q_heads), head = (int)(unit - (long long)row * p.q_heads);
+    if (row >= p.rows) return;
+    // the request that owns the row: the last i with cu_rows[i] <= row
+    int i = 0, span = p.requests;
+    while (span > 1) {
+        const int step = (span + 63) >> 6, at = i + lane * step;
+        const int hits = __popcll(__ballot(lane * step < span && p.cu_rows[at] <= row));
+        if (hits == 0) return;
+        const int left = span - (hits - 1) * step;
+        i += (hits - 1) * step;
+        span = left < step ? left : step;
+    }
+    const int r0 = p.cu_rows[i], r1 = p.cu_rows[i + 1];
+    if (r0 < 0 || r0 > row || row >= r1 || r1 > p.rows) return;
+    const int splits = (long long)(r1 - r0) * a.group.d <= a.small ? a.merge_few : a.merge_chunk;
+    if (splits == 1) return;
+    const long long stride = (long long)p.rows * p.q_heads, at = (long long)row * p.q_heads + head;
+    const float mine = lane < splits ? a.part_lse[lane * stride + at] : -INFINITY;
+    float top = mine;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+    const float w = mine == -INFINITY ? 0.f : exp2_of(mine - top);
+    float total = w;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) total += __shfl_xor(total, o, 64);
+    const int dim = p.pages.head_dim;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < splits; ++s) {
+        const float ws = __shfl(w, s, 64);
+        if (ws == 0.f) continue;                      // an empty split wrote no values
+        if (4 * lane < dim) v += *(const f32x4*)(a.part + (s * stride + at) * dim + 4 * lane) * ws;
+    }
+    const float inv = total == 0.f ? 0.f : 1.0f / total;
+    if (4 * lane < dim) {
+        x4<T> y;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) y[r] = (T)(v[r] * inv);
+        *(x4<T>*)((T*)p.out + (long long)row * p.out_row_stride + (long long)head * p.out_head_stride + 4 * lane) = y;
+    }
+    if (p.lse && lane == 0) p.lse[(long long)row * p.lse_row_stride + head] = total == 0.f ? -INFINITY : (top + __log2f(total)) * kLn2;
+}
+
+// ------------------------------------------------------------------ host
+
+constexpr int kMostSplits = 64;
+
+// Splits of the keys: enough workgroups for the chip, but no split below `least_keys` keys of the longest context known.
+int splits_for(long long groups, long long want, long long keys, int least_keys) {
+    const long long s = std::min((want + groups - 1) / groups, (keys + least_keys - 1) / least_keys);
+    return static_cast<int>(std::max(1ll, std::min<long long>(s, kMostSplits)));
+}
+
+Cut cut_of(const PttsPagedAttention& p, int cus) {
+    Cut c;
+    const long long G = p.q_heads / p.pages.kv_heads, packed = p.rows * G;
+    const bool is_float = p.q_type == PTTS_TYPE_F32;
+    const long long most_rows = p.max_rows > 0 ? std::min(p.max_rows, p.rows) : p.rows;
+    long long keys = std::max(1ll, static_cast<long long>(p.table_width) * p.pages.page_size);
+    if (p.max_kv > 0) keys = std::min<long long>(keys, p.max_kv);
+    if (p.window > 0) keys = std::min<long long>(keys, static_cast<long long>(p.window) + p.sinks + most_rows);
+    c.few = is_float || p.requests > 1 || most_rows * G <= kFewRows;
+    c.chunk = !is_float && most_rows * G > kFewRows;
+    c.few_keys = is_float ? 64 : 128;
+    if (c.few && c.chunk) { c.small = kFewRows; c.few_direct = 1; }
+    c.chunk_tiles = packed / kChunkRows + p.requests;
+    c.few_tiles = c.few_direct ? static_cast<long long>(p.requests) * c.few_direct : packed / kFewRows + p.requests;
+    if (c.chunk) {
+        const long long groups = std::max(1ll, packed / kChunkRows) * p.pages.kv_heads;
+        c.chunk_splits = splits_for(groups, groups >= cus ? groups : 2ll * cus, keys, 512);
+        c.chunk_least = static_cast<int>(std::max(1ll, (keys / kChunkKeys + c.chunk_splits - 1) / c.chunk_splits));
+    }
+    if (c.few) {
+        const long long groups = std::max<long long>(p.requests, c.small ? 0 : packed / kFewRows) * p.pages.kv_heads;
+        c.few_splits = splits_for(groups, groups >= 2ll * cus ? groups : 4ll * cus, keys, 2 * c.few_keys);
+        c.few_least = static_cast<int>(std::max(1ll, (keys / c.few_keys + c.few_splits - 1) / c.few_splits));
+    }
+    const long long most = std::max(c.chunk_splits, c.few_splits);
+    if (most > 1) c.bytes = most * p.rows * p.q_heads * (p.pages.head_dim + 1ll) * 4;
+    return c;
+}
+
+template <typename T, typename C> void launch_few(const AttnArgs& a, unsigned grid, hipStream_t s) {
+    const int d = a.p.pages.head_dim;
+    if (d <= 64) hipLaunchKernelGGL((attention_few_kernel<T, C, 64>), dim3(grid), dim3(256), 0, s, a);
+    else if (d <= 128) hipLaunchKernelGGL((attention_few_kernel<T, C, 128>), dim3(grid), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((attention_few_kernel<T, C, 256>), dim3(grid), dim3(256), 0, s, a);
+}
+template <typename T> void launch_chunk(const AttnArgs& a, unsigned grid, hipStream_t s) {
+    const int d = a.p.pages.head_dim;
+    if (d <= 64) hipLaunchKernelGGL((attention_chunk_kernel<T, 64>), dim3(grid), dim3(256), 0, s, a);
+    else if (d <= 128) hipLaunchKernelGGL((attention_chunk_kernel<T, 128>), dim3(grid), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((attention_chunk_kernel<T, 256>), dim3(grid), dim3(256), 0, s, a);
+}
+
+unsigned grid_of(long long n) {
+    if (n > 0x7fffffffll) throw std::runtime_error("paged_attention: too many rows and heads for one call");
+    return static_cast<unsigned>(n);
 }
 
 }  // namespace
@@ -123,27 +830,48 @@ void check_paged_attention(const PttsPagedAttention& p) {
         throw std::runtime_error(w + "q and out must be aligned to 16 bytes, strides too");
 }
 
-long long paged_attention_workspace(const PttsPagedAttention& p, int cus) {
-    (void)cus;
-    return 0;
-}
+long long paged_attention_workspace(const PttsPagedAttention& p, int cus) { return p.rows == 0 || p.requests == 0 ? 0 : cut_of(p, cus).bytes; }
 
 void launch_paged_attention(const PttsPagedAttention& p, int cus, hipStream_t s) {
-    (void)cus;
     if (p.rows == 0 || p.requests == 0) return;
+    const Cut c = cut_of(p, cus);
+    if (c.bytes > 0) {
+        if (!p.workspace || p.workspace_bytes < c.bytes)
+            throw std::runtime_error("paged_attention: a workspace of " + std::to_string(c.bytes) + " bytes is required");
+        if (reinterpret_cast<uintptr_t>(p.workspace) % 16) throw std::runtime_error("paged_attention: the workspace must be aligned to 16 bytes");
+    }
+    const unsigned chunk_grid = grid_of(c.chunk_tiles * c.chunk_splits * p.pages.kv_heads), few_grid = grid_of(c.few_tiles * c.few_splits * p.pages.kv_heads),
+                   merge_grid = grid_of((static_cast<long long>(p.rows) * p.q_heads + 3) / 4);
     AttnArgs a;
     a.p = p;
-    a.p.window = p.window > 1 << 30 ? 0 : p.window;   // no context is that long
+    if (p.window > 1 << 30) a.p.window = 0;          // no context is that long
     a.page = FastDiv::of(static_cast<unsigned>(p.pages.page_size));
-    a.group = p.q_heads / p.pages.kv_heads;
+    a.group = FastDiv::of(static_cast<unsigned>(p.q_heads / p.pages.kv_heads));
     a.scale2 = p.scale * 1.4426950408889634f;
-    const long long units = static_cast<long long>(p.rows) * p.q_heads;
-    if ((units + 3) / 4 > 0x7fffffffll) throw std::runtime_error("paged_attention: too many rows and heads for one call");
-    const dim3 grid(static_cast<unsigned>((units + 3) / 4)), block(256);
-    if (p.q_type == PTTS_TYPE_F32 && p.pages.type == PTTS_TYPE_BF16) hipLaunchKernelGGL((attention_rows_kernel<float, __bf16>), grid, block, 0, s, a);
-    else if (p.q_type == PTTS_TYPE_F32) hipLaunchKernelGGL((attention_rows_kernel<float, float>), grid, block, 0, s, a);
-    else if (p.q_type == PTTS_TYPE_BF16) hipLaunchKernelGGL((attention_rows_kernel<__bf16, __bf16>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((attention_rows_kernel<_Float16, _Float16>), grid, block, 0, s, a);
+    a.part = static_cast<float*>(p.workspace);
+    a.part_lse = a.part + static_cast<long long>(std::max(c.chunk_splits, c.few_splits)) * p.rows * p.q_heads * p.pages.head_dim;
+    a.small = c.small;
+    a.merge_few = c.few_splits;
+    a.merge_chunk = c.chunk ? c.chunk_splits : c.few_splits;
+    if (c.chunk) {
+        AttnArgs b = a;
+        b.tiles = c.chunk_tiles; b.splits = c.chunk_splits; b.least = c.chunk_least; b.direct = 0;
+        if (p.q_type == PTTS_TYPE_BF16) launch_chunk<__bf16>(b, chunk_grid, s);
+        else launch_chunk<_Float16>(b, chunk_grid, s);
+    }
+    if (c.few) {
+        AttnArgs b = a;
+        b.tiles = c.few_tiles; b.splits = c.few_splits; b.least = c.few_least; b.direct = c.few_direct;
+        if (p.q_type == PTTS_TYPE_F32 && p.pages.type == PTTS_TYPE_BF16) launch_few<float, __bf16>(b, few_grid, s);
+        else if (p.q_type == PTTS_TYPE_F32) launch_few<float, float>(b, few_grid, s);
+        else if (p.q_type == PTTS_TYPE_BF16) launch_few<__bf16, __bf16>(b, few_grid, s);
+        else launch_few<_Float16, _Float16>(b, few_grid, s);
+    }
+    if (c.bytes > 0) {
+        if (p.q_type == PTTS_TYPE_F32) hipLaunchKernelGGL(attention_merge_kernel<float>, dim3(merge_grid), dim3(256), 0, s, a);
+        else if (p.q_type == PTTS_TYPE_BF16) hipLaunchKernelGGL(attention_merge_kernel<__bf16>, dim3(merge_grid), dim3(256), 0, s, a);
+        else hipLaunchKernelGGL(attention_merge_kernel<_Float16>, dim3(merge_grid), dim3(256), 0, s, a);
+    }
 }
 
 }  // namespace ptts
