@@ -164,42 +164,45 @@ __device__ __forceinline__ bool none_seen(const PttsPagedAttention& p, int k0, i
     return k0 > p1 || (p.window > 0 && k1 <= p0 - p.window && k0 >= p.sinks);
 }
 
-// Element offset of a key's row under one key head, -1 where no row of the tile sees it (then it reads as zeros, so that nothing
-// stale reaches a product) or where its page id is not one.
+// What stands in for rows that are not read: keys that no row of the tile sees (so that nothing stale reaches a product) and keys
+// whose page id is not one.
+__device__ const uint4 kZeros = {0, 0, 0, 0};
+
+// The page id of a key, kUnseen where no row of the tile sees it.  The id is not looked at here, so that the load stays in flight.
+constexpr int kUnseen = -0x7fffffff;
 __device__ __forceinline__ int page_of(const AttnArgs& a, const Tile& t, const int* table, int key) {
-    if (key > t.p1 || (key < t.low && key >= a.p.sinks)) return -1;
-    const int id = table[a.page.div(key)];
-    return id >= 0 && id < a.p.pages.pages ? id : -2;
+    int id = kUnseen;
+    if (key <= t.p1 && (key >= t.low || key < a.p.sinks)) id = table[a.page.div(key)];
+    return id;
 }
-__device__ __forceinline__ long long row_at(const AttnArgs& a, int id, int key, int kvh) {
+// Element offset of a key's row under one key head, -1: not read.
+__device__ __forceinline__ long long row_at(const AttnArgs& a, int id, int key, int kvh, int& bad) {
     const PttsPages& g = a.p.pages;
-    return id < 0 ? -1 : (long long)id * g.page_stride + (long long)(key - (int)a.page.div(key) * g.page_size) * g.row_stride + (long long)kvh * g.head_stride;
+    const bool ok = id >= 0 && id < g.pages;
+    if (!ok && id != kUnseen) bad |= kStatusPage;
+    const long long at = (long long)id * g.page_stride + (long long)(key - (int)a.page.div(key) * g.page_size) * g.row_stride + (long long)kvh * g.head_stride;
+    return ok ? at : -1;
 }
 
 // Values that are NaN or infinite and stand at keys which only some rows of a tile see must not meet the other rows' zero weights.
-// Such a block is rare (it needs a block at the border of what is seen, and a value that is not finite): its values are split into
-// finite ones, which the product takes, and 0/1 marks of NaN and of the infinities, whose products with the 0/1 pattern of seen
-// keys say which sums they reach.
-template <typename T> __device__ __forceinline__ bool not_finite2(unsigned w) {
+// In blocks at the border of what is seen they are replaced by zeros on their way to the products, and a workgroup that met one
+// goes over its border blocks once more at the end and adds them, one by one, to the sums of the rows that see them (a weight is
+// positive, so a NaN or an infinity reaches the sum as it is).
+template <typename T> __device__ __forceinline__ unsigned finite_mask(unsigned w) {     // ones where a value of the word is finite
+    if constexpr (std::is_same<T, float>::value) return (w & 0x7f800000u) == 0x7f800000u ? 0u : ~0u;
     constexpr unsigned e = std::is_same<T, __bf16>::value ? 0x7f80u : 0x7c00u;
-    return (w & e) == e || ((w >> 16) & e) == e;
+    return ((w & e) == e ? 0u : 0xffffu) | (((w >> 16) & e) == e ? 0u : 0xffff0000u);
 }
-template <typename T> __device__ __forceinline__ bool not_finite(uint4 w) {
-    return not_finite2<T>(w.x) || not_finite2<T>(w.y) || not_finite2<T>(w.z) || not_finite2<T>(w.w);
-}
-// kind 0: the finite values, zero elsewhere; 1, 2, 3: ones where a value is NaN, positive, negative infinity
-template <typename T> __device__ __forceinline__ x8<T> marked(x8<T> v, int kind) {
-    x8<T> y;
+// N words cleaned; `kept` loses the bits of what was replaced
+template <typename T, int N> __device__ __forceinline__ void clean(unsigned (&w)[N], unsigned& kept) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const float f = (float)v[j], mark = (kind == 1 ? f != f : kind == 2 ? f == INFINITY : f == -INFINITY) ? 1.f : 0.f;
-        y[j] = (T)(kind == 0 ? (fabsf(f) < INFINITY ? f : 0.f) : mark);
+    for (int i = 0; i < N; ++i) {
+        const unsigned m = finite_mask<T>(w[i]);
+        w[i] &= m;
+        kept &= m;
     }
-    return y;
 }
-__device__ __forceinline__ float with_mark(float sum, float hits, int kind) {
-    return hits > 0.f ? kind == 1 ? NAN : kind == 2 ? sum + INFINITY : sum - INFINITY : sum;
-}
+__device__ __forceinline__ float add_not_finite(float sum, float v) { return fabsf(v) < INFINITY ? sum : sum + v; }
 
 // exp2 of what is at most kLag; denormals flush to zero
 __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -252,25 +255,21 @@ __global__ __launch_bounds__(256, DH == 256 ? 1 : 2) void attention_chunk_kernel
     const int* table = p.block_table + (long long)t.i * p.table_stride;
     const int unit = tid % kUnits, sr = tid / kUnits;
     const bool unit_live = unit * 8 < dim;
-    int ids[kPasses];
     uint4 kreg[kPasses], vreg[kPasses];
-    int bad = t.bad;
-    auto look_up = [&](int u) {
-        const int k0 = list.block(u) * kChunkKeys;
-#pragma unroll
-        for (int i = 0; i < kPasses; ++i) ids[i] = page_of(a, t, table, k0 + sr + kPassRows * i);
-    };
+    int bad = t.bad, id = kUnseen;
+    // Lane l of every wave looks up key l of a block, one block before its rows are read; the threads that copy the row take its
+    // place from there.
+    auto look_up = [&](int u) { id = page_of(a, t, table, list.block(u) * kChunkKeys + lane); };
     auto load = [&](int u) {
-        const int k0 = list.block(u) * kChunkKeys;
+        const long long mine = row_at(a, id, list.block(u) * kChunkKeys + lane, kvh, bad);
+        long long at[kPasses];
+#pragma unroll
+        for (int i = 0; i < kPasses; ++i) at[i] = __shfl(mine, sr + kPassRows * i, 64);
 #pragma unroll
         for (int i = 0; i < kPasses; ++i) {
-            if (ids[i] == -2) bad |= kStatusPage;
-            const long long at = row_at(a, ids[i], k0 + sr + kPassRows * i, kvh);
-            kreg[i] = vreg[i] = make_uint4(0, 0, 0, 0);
-            if (at >= 0 && unit_live) {
-                kreg[i] = *(const uint4*)((const T*)p.pages.k + at + unit * 8);
-                vreg[i] = *(const uint4*)((const T*)p.pages.v + at + unit * 8);
-            }
+            const bool ok = at[i] >= 0 && unit_live;
+            kreg[i] = *(ok ? (const uint4*)((const T*)p.pages.k + at[i] + unit * 8) : &kZeros);
+            vreg[i] = *(ok ? (const uint4*)((const T*)p.pages.v + at[i] + unit * 8) : &kZeros);
         }
     };
 
@@ -281,33 +280,30 @@ __global__ __launch_bounds__(256, DH == 256 ? 1 : 2) void attention_chunk_kernel
         for (int r = 0; r < 16; ++r) o[n][r] = 0.f;
     float top = -INFINITY, sum = 0.f;      // reference of the exponents in log2 units, this lane's part of the sum
 
-    const int ky = key_swizzle<DH>(col) ^ h;
     const int vrow = 4 * h + ((lane & 15) >> 2);
-    const T* vbase = Vs + vrow * DH + 4 * (lane & 1);
     const int vunit = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), vx = value_swizzle<DH>(vrow);
+    int kbase = col * DH * 2 + ((key_swizzle<DH>(col) ^ h) << 4), vbase = vrow * DH * 2 + 8 * (lane & 1);    // bytes
+    auto key_frag = [&](int b, int ks) {    // rows 32 b + col, head values 16 ks + 8 h ..: the swizzle is a part of kbase
+        return *(const x8<T>*)((const char*)Ks + (kbase ^ (ks << 5)) + b * 32 * DH * 2);
+    };
     auto value = [&](int n, int s) {        // V^T of 32 head values from 32 n and keys 16 s ..: keys 4 h + 0..3 and 8 + 4 h + 0..3
-        const T* at = vbase + 16 * s * DH + ((4 * n + vunit) ^ vx) * 8;
+        const char* at = (const char*)Vs + vbase + (((4 * n + vunit) ^ vx) << 4) + 16 * s * DH * 2;
         union { s16x4 w[2]; x8<T> v; } u;
         u.w[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at);
-        u.w[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(at + 8 * DH));
+        u.w[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(at + 8 * DH * 2));
         return u.v;
     };
 
-    if (u0 < u1) {
-        look_up(u0);
-        load(u0);
-        if (u0 + 1 < u1) look_up(u0 + 1);
-    }
-    for (int u = u0; u < u1; ++u) {
+    // One block.  kBorder: a block that some row of the tile does not see whole; the others need no masks.
+    unsigned kept = ~0u;
+    auto step = [&](auto border, int u) {
+        constexpr bool kBorder = decltype(border)::value;
         const int k0 = list.block(u) * kChunkKeys, k1 = k0 + kChunkKeys - 1;
-        bool odd = false;                   // values that are not finite in a block that not every row sees whole
-        if (!all_seen(p, k0, k1, t.p0, t.p1)) {
+        if constexpr (kBorder) {
 #pragma unroll
-            for (int i = 0; i < kPasses; ++i) odd |= not_finite<T>(vreg[i]);
-            odd = __builtin_amdgcn_readfirstlane(__syncthreads_or(odd));
-        } else {
-            __syncthreads();                // the previous block is consumed
+            for (int i = 0; i < kPasses; ++i) clean<T>(reinterpret_cast<unsigned(&)[4]>(vreg[i]), kept);
         }
+        __syncthreads();                    // the previous block is consumed
 #pragma unroll
         for (int i = 0; i < kPasses; ++i) {
             const int r = sr + kPassRows * i;
@@ -319,29 +315,25 @@ __global__ __launch_bounds__(256, DH == 256 ? 1 : 2) void attention_chunk_kernel
             load(u + 1);
             if (u + 2 < u1) look_up(u + 2);
         }
-        if (idle || none_seen(p, k0, k1, pw0, pw1)) continue;
+        if (idle || (kBorder && none_seen(p, k0, k1, pw0, pw1))) return;
+        asm volatile("" : "+v"(kbase));     // its variants are formed anew: kept, they would be spilled
 
         f32x16 s[2];
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
+        for (int b = 0; b < 2; ++b)
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[b][r] = 0.f;
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks)
-                s[b] = mma32(*(const x8<T>*)(Ks + (32 * b + col) * DH + ((2 * ks) ^ ky) * 8), qf[ks], s[b]);
-        }
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+            for (int b = 0; b < 2; ++b) s[b] = mma32(key_frag(b, ks), qf[ks], s[b]);
         // lane: query col; s[b][r] belongs to key k0 + 32 b + 8 (r / 4) + 4 h + r % 4
-        unsigned mask = ~0u;
-        if (!all_seen(p, k0, k1, pw0, pw1)) {
-            mask = 0;
+        if constexpr (kBorder) {
 #pragma unroll
             for (int b = 0; b < 2; ++b)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const bool ok = seen(p, k0 + 32 * b + 8 * (r >> 2) + 4 * h + (r & 3), pos);
-                    mask |= ok ? 1u << (16 * b + r) : 0u;
-                    s[b][r] = ok ? s[b][r] : -INFINITY;
-                }
+                for (int r = 0; r < 16; ++r)
+                    s[b][r] = seen(p, k0 + 32 * b + 8 * (r >> 2) + 4 * h + (r & 3), pos) ? s[b][r] : -INFINITY;
         }
         float best = s[0][0];
 #pragma unroll
@@ -368,33 +360,49 @@ __global__ __launch_bounds__(256, DH == 256 ? 1 : 2) void attention_chunk_kernel
                 sum += e;
                 w[2 * b + (r >> 3)][r & 7] = (T)e;
             }
-        if (!odd) {
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
+        for (int k = 0; k < 4; ++k)
 #pragma unroll
-                for (int k = 0; k < 4; ++k) o[n] = mma32(value(n, k), w[k], o[n]);
-        } else {
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int k = 0; k < 4; ++k) o[n] = mma32(marked(value(n, k), 0), w[k], o[n]);
-            x8<T> see[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-#pragma unroll
-                for (int j = 0; j < 8; ++j) see[k][j] = (T)((mask >> (8 * k + j)) & 1 ? 1.f : 0.f);
+            for (int n = 0; n < NT; ++n) o[n] = mma32(value(n, k), w[k], o[n]);
+    };
+
+    if (u0 < u1) {
+        look_up(u0);
+        load(u0);
+        if (u0 + 1 < u1) look_up(u0 + 1);
+    }
+    for (int u = u0; u < u1;) {
+        const int k0 = list.block(u) * kChunkKeys;
+        if (!all_seen(p, k0, k0 + kChunkKeys - 1, t.p0, t.p1)) {
+            step(std::true_type{}, u++);
+            continue;
+        }
+        // a run of whole blocks: once the last row's window has begun, all of them up to the last one that row p0 sees to its end
+        int last = u + 1;
+        if (u >= list.sink && (p.window <= 0 || k0 > t.p1 - p.window)) last = max(last, min(u1, list.sink + (t.p0 + 1) / kChunkKeys - list.start));
+        for (; u < last; ++u) step(std::false_type{}, u);
+    }
+    if (__syncthreads_or(kept != ~0u)) {
+        for (int u = u0; u < u1; ++u) {
+            const int k0 = list.block(u) * kChunkKeys;
+            if (all_seen(p, k0, k0 + kChunkKeys - 1, t.p0, t.p1)) continue;
+            look_up(u);
+            const long long mine = row_at(a, id, k0 + lane, kvh, bad);
 #pragma unroll 1
-            for (int kind = 1; kind < 4; ++kind)
+            for (int j = 0; j < kChunkKeys; ++j) {
+                const long long at = __shfl(mine, j, 64);
+                if (at < 0 || !seen(p, k0 + j, pos)) continue;
+                const T* v = (const T*)p.pages.v + at + 4 * h;
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    f32x16 c;
+                for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) c[r] = 0.f;
+                    for (int q = 0; q < 4; ++q)
+                        if (32 * n + 8 * q < dim) {
+                            const x4<T> x = *(const x4<T>*)(v + 32 * n + 8 * q);
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) c = mma32(marked(value(n, k), kind), see[k], c);
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) o[n][r] = with_mark(o[n][r], c[r], kind);
-                }
+                            for (int r = 0; r < 4; ++r) o[n][4 * q + r] = add_not_finite(o[n][4 * q + r], (float)x[r]);
+                        }
+            }
         }
     }
 
@@ -486,8 +494,7 @@ __global__ __launch_bounds__(256, DH == 256 ? 1 : 2) void attention_few_kernel(A
         const int k0 = list.block(u) * kKeys + wave * kWaveKeys;
 #pragma unroll
         for (int b = 0; b < NA; ++b) {
-            if (ids[b] == -2) bad |= kStatusPage;
-            const long long at = row_at(a, ids[b], k0 + 16 * b + li, kvh);
+            const long long at = row_at(a, ids[b], k0 + 16 * b + li, kvh, bad);
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
                 const typename S::kvec zero = {};
@@ -512,7 +519,8 @@ __global__ __launch_bounds__(256, DH == 256 ? 1 : 2) void attention_few_kernel(A
     for (int n = 0; n < CPL; ++n) o[n] = f32x4{0.f, 0.f, 0.f, 0.f};
     float top = -INFINITY, sum = 0.f;
 
-    auto work = [&](int u, const S& x) {
+    unsigned kept = ~0u;
+    auto work = [&](int u, S& x) {
         const int k0 = list.block(u) * kKeys + wave * kWaveKeys, k1 = k0 + kWaveKeys - 1;
         if (none_seen(p, k0, k1, t.p0, t.p1)) return;
         f32x4 s[NA];
@@ -533,18 +541,17 @@ __global__ __launch_bounds__(256, DH == 256 ? 1 : 2) void attention_few_kernel(A
             }
         }
         // lane: query li; s[b][r] belongs to key k0 + 16 b + 4 g + r
-        const bool whole = all_seen(p, k0, k1, t.p0, t.p1);
-        unsigned mask = ~0u;
-        if (!whole) {
-            mask = 0;
+        if (!all_seen(p, k0, k1, t.p0, t.p1)) {
 #pragma unroll
             for (int b = 0; b < NA; ++b)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const bool ok = seen(p, k0 + 16 * b + 4 * g + r, pos);
-                    mask |= ok ? 1u << (4 * b + r) : 0u;
-                    s[b][r] = ok ? s[b][r] : -INFINITY;
-                }
+                for (int r = 0; r < 4; ++r) s[b][r] = seen(p, k0 + 16 * b + 4 * g + r, pos) ? s[b][r] : -INFINITY;
+            if (t.p0 != t.p1) {            // rows of one position see the same keys, and what they do not see was not read
+#pragma unroll
+                for (int r = 0; r < 4 * NA; ++r)
+#pragma unroll
+                    for (int n = 0; n < VN; ++n) clean<C>(reinterpret_cast<unsigned(&)[sizeof(C) * VW / 4]>(x.v[r][n]), kept);
+            }
         }
         float best = s[0][0];
 #pragma unroll
@@ -568,41 +575,15 @@ __global__ __launch_bounds__(256, DH == 256 ? 1 : 2) void attention_few_kernel(A
                 e[4 * b + r] = exp2_of(__builtin_fmaf(s[b][r], a.scale2, -base));
                 sum += e[4 * b + r];
             }
-        // values that are not finite at keys that not every row of the tile sees
-        bool odd = false;
-        if (!whole && t.p0 != t.p1) {
-#pragma unroll
-            for (int r = 0; r < 4 * NA; ++r)
-#pragma unroll
-                for (int n = 0; n < VN; ++n)
-#pragma unroll
-                    for (int j = 0; j < VW; ++j) odd |= !(fabsf((float)x.v[r][n][j]) < INFINITY);
-            odd = __builtin_amdgcn_readfirstlane(__any(odd));
-        }
         if constexpr (kFloat) {
 #pragma unroll
-            for (int n = 0; n < CPL; ++n) {
-                f32x4 cn = {0.f, 0.f, 0.f, 0.f}, cu = cn, cd = cn;
+            for (int n = 0; n < CPL; ++n)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    float v = (float)x.v[r][n / VW][n % VW];
-                    if (odd) {
-                        const float see = (mask >> r) & 1 ? 1.f : 0.f;
-                        cn = __builtin_amdgcn_mfma_f32_16x16x4f32(v != v ? 1.f : 0.f, see, cn, 0, 0, 0);
-                        cu = __builtin_amdgcn_mfma_f32_16x16x4f32(v == INFINITY ? 1.f : 0.f, see, cu, 0, 0, 0);
-                        cd = __builtin_amdgcn_mfma_f32_16x16x4f32(v == -INFINITY ? 1.f : 0.f, see, cd, 0, 0, 0);
-                        if (!(fabsf(v) < INFINITY)) v = 0.f;
-                    }
-                    o[n] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, e[r], o[n], 0, 0, 0);
-                }
-                if (odd)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) o[n][r] = with_mark(with_mark(with_mark(o[n][r], cn[r], 1), cu[r], 2), cd[r], 3);
-            }
+                for (int r = 0; r < 4; ++r) o[n] = __builtin_amdgcn_mfma_f32_16x16x4f32((float)x.v[r][n / VW][n % VW], e[r], o[n], 0, 0, 0);
         } else {
-            x8<T> w, see;
+            x8<T> w;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) { w[j] = (T)e[j]; see[j] = (T)((mask >> j) & 1 ? 1.f : 0.f); }
+            for (int j = 0; j < 8; ++j) w[j] = (T)e[j];
 #pragma unroll
             for (int n = 0; n < CPL; ++n) {
                 // column n of the eight rows: halves of their registers put together in pairs
@@ -614,17 +595,7 @@ __global__ __launch_bounds__(256, DH == 256 ? 1 : 2) void attention_few_kernel(A
                     hi.v = x.v[2 * j + 1][n / VW];
                     u.d[j] = __builtin_amdgcn_perm(hi.d[n % VW / 2], lo.d[n % VW / 2], n & 1 ? 0x07060302u : 0x05040100u);
                 }
-                if (!odd) {
-                    o[n] = mma16(u.v, w, o[n]);
-                } else {
-                    o[n] = mma16(marked(u.v, 0), w, o[n]);
-#pragma unroll 1
-                    for (int kind = 1; kind < 4; ++kind) {
-                        const f32x4 c = mma16(marked(u.v, kind), see, f32x4{0.f, 0.f, 0.f, 0.f});
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) o[n][r] = with_mark(o[n][r], c[r], kind);
-                    }
-                }
+                o[n] = mma16(u.v, w, o[n]);
             }
         }
     };
@@ -647,6 +618,28 @@ __global__ __launch_bounds__(256, DH == 256 ? 1 : 2) void attention_few_kernel(A
                 if (u + 3 < u1) look_up(u + 3);
             }
             work(u + 1, two);
+        }
+    }
+    if (__any(kept != ~0u)) {
+        for (int u = u0; u < u1; ++u) {
+            const int k0 = list.block(u) * kKeys + wave * kWaveKeys;
+            if (all_seen(p, k0, k0 + kWaveKeys - 1, t.p0, t.p1) || none_seen(p, k0, k0 + kWaveKeys - 1, t.p0, t.p1)) continue;
+            look_up(u);
+#pragma unroll
+            for (int b = 0; b < NA; ++b) {
+                const long long mine = row_at(a, ids[b], k0 + 16 * b + li, kvh, bad);
+#pragma unroll 1
+                for (int j = 0; j < 16; ++j) {
+                    const long long at = __shfl(mine, j, 64);
+                    if (at < 0 || !seen(p, k0 + 16 * b + j, pos)) continue;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+#pragma unroll
+                        for (int n = 0; n < CPL; ++n)
+                            if (CPL * (4 * g + r) + n < dim)
+                                o[n][r] = add_not_finite(o[n][r], (float)((const C*)p.pages.v)[at + CPL * (4 * g + r) + n]);
+                }
+            }
         }
     }
     if (bad && p.status) atomicOr(p.status, bad);
