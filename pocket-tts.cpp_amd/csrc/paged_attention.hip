@@ -1,12 +1,14 @@
 // Attention of every request's new rows over its pages (pocket_tts_amd.h, ptts_paged_attention).
 //
 // The G query heads of a key head share its keys, so the rows of one request and one key head are packed: packed row m is new
-// row m / G under head m % G.  Three kernels work on tiles of packed rows:
+// row m / G under head m % G.  Two forms work on tiles of packed rows:
 //
 //   chunk   128 packed rows, four waves of 32; key blocks of 64 go through LDS and are read by all four waves
 //   few     16 packed rows; four waves walk different keys straight from memory and join at the end (single tokens: bound by
 //           the one read of the keys and values)
-//   merge   joins the parts of rows whose keys were cut into splits
+//   merge   joins the results of rows whose keys were cut into splits
+//
+// Batches that may hold both kinds of requests run both forms in one launch, the memory-bound one beside the other.
 //
 // All products are formed transposed, S^T = K Q^T and O^T = V^T P^T, so that a lane keeps one query for the whole kernel (its
 // running maximum and sum are scalars of the lane) and the weights leave the first product in the layout the second one takes
@@ -31,15 +33,14 @@ constexpr int kChunkRows = 128, kChunkKeys = 64;   // chunk kernel: packed rows 
 constexpr int kFewRows = 16;                       // few kernel: packed rows of a workgroup
 constexpr float kLn2 = 0.69314718055994531f, kLag = 8.0f;
 
-// How a call is cut: which kernels run, over how many tiles, into how many splits of the keys.
+// How a call is cut: which forms run, over how many tiles, into how many splits of the keys.
 struct Cut {
     bool chunk = false, few = false;
-    int small = 0;              // both kernels run: requests of at most this many packed rows go to the few kernel
-    int few_direct = 0;         // ... which then gives each request this many tiles; 0: tiles are found by search
-    int few_keys = 0;           // keys of one step of a workgroup of the few kernel
+    int small = 0;              // both run: requests of at most this many packed rows (one tile) go to the few form
     long long chunk_tiles = 0, few_tiles = 0;
     int chunk_splits = 1, few_splits = 1;
-    int chunk_least = 1, few_least = 1;   // fewest key blocks of a split
+    int chunk_least = 1, few_least = 1;               // fewest key blocks of a split
+    long long chunk_parts = 0, few_parts = 0;         // rows of one split's results in the workspace
     long long bytes = 0;
 };
 
@@ -47,11 +48,13 @@ struct AttnArgs {
     PttsPagedAttention p;
     FastDiv page, group;
     float scale2;               // scale * log2(e)
-    long long tiles;            // of the kernel that is launched
-    int splits, least, small, direct;
-    int merge_few, merge_chunk; // splits of the two kernels' rows (merge)
-    float* part;                // [split][row][head][dim], then [split][row][head] of log2 sum exp2
-    float* part_lse;
+    int small;
+    unsigned few_blocks;        // workgroups of the few form; those of the chunk form follow
+    long long chunk_tiles;
+    int chunk_splits, few_splits, chunk_least, few_least;
+    // results of splits: [split][row][dim] values, normalised by the split's own sum, and [split][row] of log2 sum exp2
+    float *chunk_part, *chunk_lse, *few_part, *few_lse;
+    long long chunk_parts, few_parts;
 };
 
 typedef __attribute__((ext_vector_type(4))) float f32x4;
@@ -94,13 +97,14 @@ struct Tile {
 
 // Tile numbers of request i begin at cu_rows[i] * G / BM + i: its ceil(n G / BM) tiles end before those of the next request
 // begin, so a tile finds its request without prefix sums, 64 requests at a time, and a few numbers stay unused.
-__device__ __forceinline__ bool find_tile(const AttnArgs& a, long long tile, int rows_per_tile, Tile& t) {
+// `direct`: tile i is request i's first.
+__device__ __forceinline__ bool find_tile(const AttnArgs& a, long long tile, int rows_per_tile, bool direct, Tile& t) {
     const PttsPagedAttention& p = a.p;
     const int lane = threadIdx.x & 63, G = a.group.d;
     int sub;
-    if (a.direct) {
-        t.i = (int)(tile / a.direct);
-        sub = (int)(tile - (long long)t.i * a.direct);
+    if (direct) {
+        t.i = (int)tile;
+        sub = 0;
     } else {
         int lo = 0, span = p.requests;
         while (span > 1) {
@@ -164,10 +168,6 @@ __device__ __forceinline__ bool none_seen(const PttsPagedAttention& p, int k0, i
     return k0 > p1 || (p.window > 0 && k1 <= p0 - p.window && k0 >= p.sinks);
 }
 
-// What stands in for rows that are not read: keys that no row of the tile sees (so that nothing stale reaches a product) and keys
-// whose page id is not one.
-__device__ const uint4 kZeros = {0, 0, 0, 0};
-
 // The page id of a key, kUnseen where no row of the tile sees it.  The id is not looked at here, so that the load stays in flight.
 constexpr int kUnseen = -0x7fffffff;
 __device__ __forceinline__ int page_of(const AttnArgs& a, const Tile& t, const int* table, int key) {
@@ -175,13 +175,14 @@ __device__ __forceinline__ int page_of(const AttnArgs& a, const Tile& t, const i
     if (key <= t.p1 && (key >= t.low || key < a.p.sinks)) id = table[a.page.div(key)];
     return id;
 }
-// Element offset of a key's row under one key head, -1: not read.
-__device__ __forceinline__ long long row_at(const AttnArgs& a, int id, int key, int kvh, int& bad) {
+// Element offset of a key's row under one key head.  Rows that are not read (no row of the tile sees the key, or its page id is
+// not one) have offset 0, inside the pool, and ok false: what is loaded there is replaced by zeros.
+__device__ __forceinline__ long long row_at(const AttnArgs& a, int id, int key, int kvh, int& bad, bool& ok) {
     const PttsPages& g = a.p.pages;
-    const bool ok = id >= 0 && id < g.pages;
+    ok = id >= 0 && id < g.pages;
     if (!ok && id != kUnseen) bad |= kStatusPage;
     const long long at = (long long)id * g.page_stride + (long long)(key - (int)a.page.div(key) * g.page_size) * g.row_stride + (long long)kvh * g.head_stride;
-    return ok ? at : -1;
+    return ok ? at : 0;
 }
 
 // Values that are NaN or infinite and stand at keys which only some rows of a tile see must not meet the other rows' zero weights.
@@ -215,25 +216,27 @@ __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2
 template <int DH> __device__ __forceinline__ int key_swizzle(int row) { return DH >= 128 ? row & 15 : (row >> 1) & 7; }
 template <int DH> __device__ __forceinline__ int value_swizzle(int row) { return DH >= 128 ? (row & 3) << 2 : ((row >> 1) & 1) << 2; }
 
-template <typename T, int DH>
-__global__ __launch_bounds__(256, DH == 256 ? 1 : 2) void attention_chunk_kernel(AttnArgs a) {
+template <typename T, int DH> struct ChunkLds {
+    T k[kChunkKeys * DH], v[kChunkKeys * DH];
+};
+
+template <typename T, int DH> __device__ __forceinline__ void chunk_body(const AttnArgs& a, unsigned block, ChunkLds<T, DH>& lds) {
     constexpr int kUnits = DH / 8, kPassRows = 256 / kUnits, kPasses = kChunkKeys / kPassRows, KS = DH / 16, NT = DH / 32;
-    __shared__ __attribute__((aligned(16))) T Ks[kChunkKeys * DH];
-    __shared__ __attribute__((aligned(16))) T Vs[kChunkKeys * DH];
+    T *const Ks = lds.k, *const Vs = lds.v;
     const PttsPagedAttention& p = a.p;
     const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);   // matrix instructions ignore the lane mask: every branch around one is scalar
     // key heads first (neighbouring workgroups go to different dies, so a die's cache sees few heads), and the tiles that see
     // most keys first
-    const int kvh = blockIdx.x % p.pages.kv_heads;
-    const unsigned rest = blockIdx.x / p.pages.kv_heads;
-    const int split = rest % a.splits;
+    const int kvh = block % p.pages.kv_heads;
+    const unsigned rest = block / p.pages.kv_heads;
+    const int splits = a.chunk_splits, split = rest % splits;
     Tile t;
-    if (!find_tile(a, a.tiles - 1 - rest / a.splits, kChunkRows, t)) return;
+    if (!find_tile(a, a.chunk_tiles - 1 - rest / splits, kChunkRows, 0, t)) return;
     const int G = a.group.d, dim = p.pages.head_dim;
     if ((long long)t.n * G <= a.small) return;
     const Blocks list(t, p.sinks, kChunkKeys);
-    const int per = max(a.least, (list.count + a.splits - 1) / a.splits);
+    const int per = max(a.chunk_least, (list.count + splits - 1) / splits);
     const int u0 = split * per, u1 = min(list.count, u0 + per);
 
     // this lane's query, and the positions of this wave's rows
@@ -256,20 +259,26 @@ __global__ __launch_bounds__(256, DH == 256 ? 1 : 2) void attention_chunk_kernel
     const int unit = tid % kUnits, sr = tid / kUnits;
     const bool unit_live = unit * 8 < dim;
     uint4 kreg[kPasses], vreg[kPasses];
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i) kreg[i] = vreg[i] = make_uint4(0, 0, 0, 0);    // units behind the head's values stay zero
     int bad = t.bad, id = kUnseen;
+    unsigned long long holes = 0;           // keys of the block on its way that were not read
     // Lane l of every wave looks up key l of a block, one block before its rows are read; the threads that copy the row take its
     // place from there.
     auto look_up = [&](int u) { id = page_of(a, t, table, list.block(u) * kChunkKeys + lane); };
     auto load = [&](int u) {
-        const long long mine = row_at(a, id, list.block(u) * kChunkKeys + lane, kvh, bad);
+        bool ok;
+        const long long mine = row_at(a, id, list.block(u) * kChunkKeys + lane, kvh, bad, ok);
+        holes = __ballot(!ok);
         long long at[kPasses];
 #pragma unroll
-        for (int i = 0; i < kPasses; ++i) at[i] = __shfl(mine, sr + kPassRows * i, 64);
+        for (int i = 0; i < kPasses; ++i) at[i] = __shfl(mine, sr + kPassRows * i, 64) + unit * 8;
+        if (unit_live) {
 #pragma unroll
-        for (int i = 0; i < kPasses; ++i) {
-            const bool ok = at[i] >= 0 && unit_live;
-            kreg[i] = *(ok ? (const uint4*)((const T*)p.pages.k + at[i] + unit * 8) : &kZeros);
-            vreg[i] = *(ok ? (const uint4*)((const T*)p.pages.v + at[i] + unit * 8) : &kZeros);
+            for (int i = 0; i < kPasses; ++i) {
+                kreg[i] = *(const uint4*)((const T*)p.pages.k + at[i]);
+                vreg[i] = *(const uint4*)((const T*)p.pages.v + at[i]);
+            }
         }
     };
 
@@ -294,12 +303,21 @@ __global__ __launch_bounds__(256, DH == 256 ? 1 : 2) void attention_chunk_kernel
         return u.v;
     };
 
-    // One block.  kBorder: a block that some row of the tile does not see whole; the others need no masks.
     unsigned kept = ~0u;
-    auto step = [&](auto border, int u) {
-        constexpr bool kBorder = decltype(border)::value;
+    if (u0 < u1) {
+        look_up(u0);
+        load(u0);
+        if (u0 + 1 < u1) look_up(u0 + 1);
+    }
+    for (int u = u0; u < u1; ++u) {
         const int k0 = list.block(u) * kChunkKeys, k1 = k0 + kChunkKeys - 1;
-        if constexpr (kBorder) {
+        const bool border = !all_seen(p, k0, k1, t.p0, t.p1);       // some row of the tile does not see the block whole
+        if (holes) {
+#pragma unroll
+            for (int i = 0; i < kPasses; ++i)
+                if ((holes >> (sr + kPassRows * i)) & 1) kreg[i] = vreg[i] = make_uint4(0, 0, 0, 0);
+        }
+        if (border) {
 #pragma unroll
             for (int i = 0; i < kPasses; ++i) clean<T>(reinterpret_cast<unsigned(&)[4]>(vreg[i]), kept);
         }
@@ -315,7 +333,7 @@ __global__ __launch_bounds__(256, DH == 256 ? 1 : 2) void attention_chunk_kernel
             load(u + 1);
             if (u + 2 < u1) look_up(u + 2);
         }
-        if (idle || (kBorder && none_seen(p, k0, k1, pw0, pw1))) return;
+        if (idle || (border && none_seen(p, k0, k1, pw0, pw1))) continue;
         asm volatile("" : "+v"(kbase));     // its variants are formed anew: kept, they would be spilled
 
         f32x16 s[2];
@@ -327,13 +345,20 @@ __global__ __launch_bounds__(256, DH == 256 ? 1 : 2) void attention_chunk_kernel
         for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
             for (int b = 0; b < 2; ++b) s[b] = mma32(key_frag(b, ks), qf[ks], s[b]);
+        __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);
+#pragma unroll
+        for (int i = 0; i < KS - 3; ++i) { __builtin_amdgcn_sched_group_barrier(0x8, 2, 0); __builtin_amdgcn_sched_group_barrier(0x100, 2, 0); }
+        __builtin_amdgcn_sched_group_barrier(0x8, 6, 0);
         // lane: query col; s[b][r] belongs to key k0 + 32 b + 8 (r / 4) + 4 h + r % 4
-        if constexpr (kBorder) {
+        if (border) {
+            const int mine = k0 + 4 * h, up = pos - mine, from = p.window > 0 ? up - p.window : -1, sink = p.sinks - mine;
 #pragma unroll
             for (int b = 0; b < 2; ++b)
 #pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    s[b][r] = seen(p, k0 + 32 * b + 8 * (r >> 2) + 4 * h + (r & 3), pos) ? s[b][r] : -INFINITY;
+                for (int r = 0; r < 16; ++r) {
+                    const int c = 32 * b + 8 * (r >> 2) + (r & 3);           // seen(p, mine + c, pos)
+                    s[b][r] = c <= up && (c > from || c < sink) ? s[b][r] : -INFINITY;
+                }
         }
         float best = s[0][0];
 #pragma unroll
@@ -364,34 +389,19 @@ __global__ __launch_bounds__(256, DH == 256 ? 1 : 2) void attention_chunk_kernel
         for (int k = 0; k < 4; ++k)
 #pragma unroll
             for (int n = 0; n < NT; ++n) o[n] = mma32(value(n, k), w[k], o[n]);
-    };
-
-    if (u0 < u1) {
-        look_up(u0);
-        load(u0);
-        if (u0 + 1 < u1) look_up(u0 + 1);
-    }
-    for (int u = u0; u < u1;) {
-        const int k0 = list.block(u) * kChunkKeys;
-        if (!all_seen(p, k0, k0 + kChunkKeys - 1, t.p0, t.p1)) {
-            step(std::true_type{}, u++);
-            continue;
-        }
-        // a run of whole blocks: once the last row's window has begun, all of them up to the last one that row p0 sees to its end
-        int last = u + 1;
-        if (u >= list.sink && (p.window <= 0 || k0 > t.p1 - p.window)) last = max(last, min(u1, list.sink + (t.p0 + 1) / kChunkKeys - list.start));
-        for (; u < last; ++u) step(std::false_type{}, u);
     }
     if (__syncthreads_or(kept != ~0u)) {
         for (int u = u0; u < u1; ++u) {
             const int k0 = list.block(u) * kChunkKeys;
             if (all_seen(p, k0, k0 + kChunkKeys - 1, t.p0, t.p1)) continue;
             look_up(u);
-            const long long mine = row_at(a, id, k0 + lane, kvh, bad);
+            bool ok;
+            const long long mine = row_at(a, id, k0 + lane, kvh, bad, ok);
+            const unsigned long long there = __ballot(ok);
 #pragma unroll 1
             for (int j = 0; j < kChunkKeys; ++j) {
                 const long long at = __shfl(mine, j, 64);
-                if (at < 0 || !seen(p, k0 + j, pos)) continue;
+                if (!((there >> j) & 1) || !seen(p, k0 + j, pos)) continue;
                 const T* v = (const T*)p.pages.v + at + 4 * h;
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
@@ -410,7 +420,7 @@ __global__ __launch_bounds__(256, DH == 256 ? 1 : 2) void attention_chunk_kernel
     sum = sum_half(sum);
     if (!live) return;
     const float inv = sum == 0.f ? 0.f : 1.0f / sum, lse2 = sum == 0.f ? -INFINITY : top + __log2f(sum);
-    if (a.splits == 1) {
+    if (splits == 1) {
         T* out = (T*)p.out + (long long)row * p.out_row_stride + (long long)head * p.out_head_stride + 4 * h;
 #pragma unroll
         for (int n = 0; n < NT; ++n)
@@ -424,8 +434,8 @@ __global__ __launch_bounds__(256, DH == 256 ? 1 : 2) void attention_chunk_kernel
                 }
         if (p.lse && h == 0) p.lse[(long long)row * p.lse_row_stride + head] = lse2 * kLn2;
     } else {
-        const long long at = ((long long)split * p.rows + row) * p.q_heads + head;
-        float* part = a.part + at * dim + 4 * h;
+        const long long at = split * a.chunk_parts + (long long)row * p.q_heads + head;
+        float* part = a.chunk_part + at * dim + 4 * h;
         if (sum != 0.f)
 #pragma unroll
             for (int n = 0; n < NT; ++n)
@@ -433,7 +443,7 @@ __global__ __launch_bounds__(256, DH == 256 ? 1 : 2) void attention_chunk_kernel
                 for (int q = 0; q < 4; ++q)
                     if (32 * n + 8 * q < dim)
                         *(f32x4*)(part + 32 * n + 8 * q) = f32x4{o[n][4 * q] * inv, o[n][4 * q + 1] * inv, o[n][4 * q + 2] * inv, o[n][4 * q + 3] * inv};
-        if (h == 0) a.part_lse[at] = lse2;
+        if (h == 0) a.chunk_lse[at] = lse2;
     }
 }
 
@@ -452,25 +462,29 @@ template <typename T, typename C, int DH> struct Step {
     vvec v[4 * NA][VN];
 };
 
-template <typename T, typename C, int DH>
-__global__ __launch_bounds__(256, DH == 256 ? 1 : 2) void attention_few_kernel(AttnArgs a) {
+template <int DH> struct FewLds {
+    float joined[4][kFewRows][DH + 4];      // +4: the waves' columns of one row do not meet in one bank
+    float tops[4][kFewRows], sums[4][kFewRows];
+};
+
+template <typename T, typename C, int DH> __device__ __forceinline__ void few_body(const AttnArgs& a, unsigned block, FewLds<DH>& lds) {
     using S = Step<T, C, DH>;
     constexpr int NA = S::NA, CPL = S::CPL, KS = S::KS, KW = S::KW, VW = S::VW, VN = S::VN, kWaveKeys = 16 * NA, kKeys = 4 * kWaveKeys;
     constexpr bool kFloat = S::kFloat;
-    __shared__ float joined[4][kFewRows][DH + 4];      // +4: the waves' columns of one row do not meet in one bank
-    __shared__ float tops[4][kFewRows], sums[4][kFewRows];
+    auto &joined = lds.joined;
+    auto &tops = lds.tops, &sums = lds.sums;
     const PttsPagedAttention& p = a.p;
     const int tid = threadIdx.x, lane = tid & 63, li = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);   // matrix instructions ignore the lane mask: every branch around one is scalar
-    const int kvh = blockIdx.x % p.pages.kv_heads;
-    const unsigned rest = blockIdx.x / p.pages.kv_heads;
-    const int split = rest % a.splits;
+    const int kvh = block % p.pages.kv_heads;
+    const unsigned rest = block / p.pages.kv_heads;
+    const int splits = a.few_splits, split = rest % splits;
     Tile t;
-    if (!find_tile(a, rest / a.splits, kFewRows, t)) return;
+    if (!find_tile(a, rest / splits, kFewRows, a.small > 0, t)) return;
     const int G = a.group.d, dim = p.pages.head_dim;
     if (a.small > 0 && (long long)t.n * G > a.small) return;
     const Blocks list(t, p.sinks, kKeys);
-    const int per = max(a.least, (list.count + a.splits - 1) / a.splits);
+    const int per = max(a.few_least, (list.count + splits - 1) / splits);
     const int u0 = split * per, u1 = min(list.count, u0 + per);
 
     const int m = min(t.m0 + li, t.m1 - 1), tok = a.group.div(m), head = kvh * G + m - tok * G, row = t.row0 + tok, pos = t.pos0 + tok;
@@ -494,12 +508,14 @@ __global__ __launch_bounds__(256, DH == 256 ? 1 : 2) void attention_few_kernel(A
         const int k0 = list.block(u) * kKeys + wave * kWaveKeys;
 #pragma unroll
         for (int b = 0; b < NA; ++b) {
-            const long long at = row_at(a, ids[b], k0 + 16 * b + li, kvh, bad);
+            bool ok;
+            const long long at = row_at(a, ids[b], k0 + 16 * b + li, kvh, bad, ok);
+            const unsigned there = (unsigned)__ballot(ok);             // keys li of lanes 0 .. 15
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
                 const typename S::kvec zero = {};
                 const int d = 4 * KW * ks + KW * g;
-                x.k[b][ks] = at >= 0 && d < dim ? *(const typename S::kvec*)((const C*)p.pages.k + at + d) : zero;
+                x.k[b][ks] = ok && d < dim ? *(const typename S::kvec*)((const C*)p.pages.k + at + d) : zero;
             }
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
@@ -508,7 +524,7 @@ __global__ __launch_bounds__(256, DH == 256 ? 1 : 2) void attention_few_kernel(A
                 for (int n = 0; n < VN; ++n) {
                     const typename S::vvec zero = {};
                     const int d = CPL * li + VW * n;
-                    x.v[4 * b + r][n] = from >= 0 && d < dim ? *(const typename S::vvec*)((const C*)p.pages.v + from + d) : zero;
+                    x.v[4 * b + r][n] = ((there >> (4 * g + r)) & 1) && d < dim ? *(const typename S::vvec*)((const C*)p.pages.v + from + d) : zero;
                 }
             }
         }
@@ -627,11 +643,13 @@ __global__ __launch_bounds__(256, DH == 256 ? 1 : 2) void attention_few_kernel(A
             look_up(u);
 #pragma unroll
             for (int b = 0; b < NA; ++b) {
-                const long long mine = row_at(a, ids[b], k0 + 16 * b + li, kvh, bad);
+                bool ok;
+                const long long mine = row_at(a, ids[b], k0 + 16 * b + li, kvh, bad, ok);
+                const unsigned there = (unsigned)__ballot(ok);
 #pragma unroll 1
                 for (int j = 0; j < 16; ++j) {
                     const long long at = __shfl(mine, j, 64);
-                    if (at < 0 || !seen(p, k0 + 16 * b + j, pos)) continue;
+                    if (!((there >> j) & 1) || !seen(p, k0 + 16 * b + j, pos)) continue;
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
 #pragma unroll
@@ -675,30 +693,84 @@ __global__ __launch_bounds__(256, DH == 256 ? 1 : 2) void attention_few_kernel(A
         const float inv = total == 0.f ? 0.f : 1.0f / total, lse2 = total == 0.f ? -INFINITY : big + __log2f(total);
         const int mq = t.m0 + q, tq = a.group.div(mq), hq = kvh * G + mq - tq * G;
         const long long rq = t.row0 + tq;
-        if (a.splits == 1) {
+        if (splits == 1) {
             x4<T> w;
 #pragma unroll
             for (int r = 0; r < 4; ++r) w[r] = (T)(total == 0.f ? 0.f : v[r] * inv);
             *(x4<T>*)((T*)p.out + rq * p.out_row_stride + (long long)hq * p.out_head_stride + d) = w;
             if (p.lse && d == 0) p.lse[rq * p.lse_row_stride + hq] = lse2 * kLn2;
         } else {
-            const long long at = ((long long)split * p.rows + rq) * p.q_heads + hq;
-            if (total != 0.f) *(f32x4*)(a.part + at * dim + d) = v * inv;
-            if (d == 0) a.part_lse[at] = lse2;
+            const long long at = split * a.few_parts + (a.small > 0 ? ((long long)t.i * p.pages.kv_heads + kvh) * kFewRows + mq : rq * p.q_heads + hq);
+            if (total != 0.f) *(f32x4*)(a.few_part + at * dim + d) = v * inv;
+            if (d == 0) a.few_lse[at] = lse2;
         }
     }
 }
 
+// The forms' entries.  A launch of the few form alone does not carry the chunk form's registers and LDS.
+template <typename T, typename C, int DH> __global__ __launch_bounds__(256, DH == 256 ? 1 : 2) void attention_few_kernel(AttnArgs a) {
+    __shared__ __attribute__((aligned(16))) FewLds<DH> lds;
+    few_body<T, C, DH>(a, blockIdx.x, lds);
+}
+// Three workgroups per CU where the head fits (170 registers), else two.
+template <typename T, int DH> __global__ __launch_bounds__(256, DH == 256 ? 1 : DH == 128 ? 2 : 3) void attention_chunk_kernel(AttnArgs a) {
+    __shared__ __attribute__((aligned(16))) ChunkLds<T, DH> lds;
+    chunk_body<T, DH>(a, blockIdx.x, lds);
+}
+template <typename T, int DH> __global__ __launch_bounds__(256, DH == 256 ? 1 : DH == 128 ? 2 : 3) void attention_both_kernel(AttnArgs a) {
+    __shared__ __attribute__((aligned(16))) union Lds {
+        ChunkLds<T, DH> chunk;
+        FewLds<DH> few;
+        __device__ Lds() {}
+    } lds;
+    if (blockIdx.x < a.few_blocks) few_body<T, T, DH>(a, blockIdx.x, lds.few);
+    else chunk_body<T, DH>(a, blockIdx.x - a.few_blocks, lds.chunk);
+}
+
 // ------------------------------------------------------------------ merge
 
-// One wave per (row, head): out = sum over splits of exp2(lse_s - lse) part_s.
+// out = sum over splits of exp2(lse_s - lse) part_s, four values a thread.
 template <typename T>
-__global__ __launch_bounds__(256) void attention_merge_kernel(AttnArgs a) {
+__device__ __forceinline__ void merge_one(const PttsPagedAttention& p, const float* part, const float* lse, long long stride, int splits, long long at, long long row,
+                                          int head, int d) {
+    float top = -INFINITY;
+    for (int s = 0; s < splits; ++s) top = fmaxf(top, lse[s * stride + at]);
+    float total = 0.f;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < splits; ++s) {
+        const float l = lse[s * stride + at];
+        if (l == -INFINITY) continue;                 // nothing seen there, and no values written
+        const float w = exp2_of(l - top);
+        total += w;
+        v += *(const f32x4*)(part + (s * stride + at) * p.pages.head_dim + d) * w;
+    }
+    const float inv = total == 0.f ? 0.f : 1.0f / total;
+    x4<T> y;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) y[r] = (T)(v[r] * inv);
+    *(x4<T>*)((T*)p.out + row * p.out_row_stride + (long long)head * p.out_head_stride + d) = y;
+    if (p.lse && d == 0) p.lse[row * p.lse_row_stride + head] = total == 0.f ? -INFINITY : (top + __log2f(total)) * kLn2;
+}
+
+// Workgroups (x) 0 .. request_blocks - 1: the few form's one tile of a request (both forms ran); the others: one row each.  Workgroups
+// along y share a row's heads.
+template <typename T>
+__global__ __launch_bounds__(256) void attention_merge_kernel(AttnArgs a, unsigned request_blocks, int row_splits, const float* row_part, const float* row_lse, long long row_parts) {
     const PttsPagedAttention& p = a.p;
-    const int lane = threadIdx.x & 63;
-    const long long unit = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int row = (int)(unit / p.q_heads), head = (int)(unit - (long long)row * p.q_heads);
-    if (row >= p.rows) return;
+    const int G = a.group.d, quads = p.pages.head_dim / 4;
+    if (blockIdx.x < request_blocks) {
+        const int i = blockIdx.x, r0 = p.cu_rows[i], r1 = p.cu_rows[i + 1];
+        if (r0 < 0 || r1 > p.rows || r1 <= r0 || (long long)(r1 - r0) * G > a.small) return;
+        const int packed = (r1 - r0) * G, n = packed * p.pages.kv_heads * quads;
+        const int x = blockIdx.y * 256 + threadIdx.x;
+        if (x < n) {
+            const int q = x / quads, kvh = q / packed, m = q - kvh * packed, tok = a.group.div(m);
+            merge_one<T>(p, a.few_part, a.few_lse, a.few_parts, a.few_splits, ((long long)i * p.pages.kv_heads + kvh) * kFewRows + m, r0 + tok, kvh * G + m - tok * G,
+                         4 * (x - q * quads));
+        }
+        return;
+    }
+    const int lane = threadIdx.x & 63, row = blockIdx.x - request_blocks;
     // the request that owns the row: the last i with cu_rows[i] <= row
     int i = 0, span = p.requests;
     while (span > 1) {
@@ -710,48 +782,22 @@ __global__ __launch_bounds__(256) void attention_merge_kernel(AttnArgs a) {
         span = left < step ? left : step;
     }
     const int r0 = p.cu_rows[i], r1 = p.cu_rows[i + 1];
-    if (r0 < 0 || r0 > row || row >= r1 || r1 > p.rows) return;
-    const int splits = (long long)(r1 - r0) * a.group.d <= a.small ? a.merge_few : a.merge_chunk;
-    if (splits == 1) return;
-    const long long stride = (long long)p.rows * p.q_heads, at = (long long)row * p.q_heads + head;
-    const float mine = lane < splits ? a.part_lse[lane * stride + at] : -INFINITY;
-    float top = mine;
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
-    const float w = mine == -INFINITY ? 0.f : exp2_of(mine - top);
-    float total = w;
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) total += __shfl_xor(total, o, 64);
-    const int dim = p.pages.head_dim;
-    f32x4 v = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < splits; ++s) {
-        const float ws = __shfl(w, s, 64);
-        if (ws == 0.f) continue;                      // an empty split wrote no values
-        if (4 * lane < dim) v += *(const f32x4*)(a.part + (s * stride + at) * dim + 4 * lane) * ws;
+    if (r0 < 0 || r0 > row || row >= r1 || r1 > p.rows || (long long)(r1 - r0) * G <= a.small) return;
+    const int x = blockIdx.y * 256 + threadIdx.x;
+    if (x < p.q_heads * quads) {
+        const int head = x / quads;
+        merge_one<T>(p, row_part, row_lse, row_parts, row_splits, (long long)row * p.q_heads + head, row, head, 4 * (x - head * quads));
     }
-    const float inv = total == 0.f ? 0.f : 1.0f / total;
-    if (4 * lane < dim) {
-        x4<T> y;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) y[r] = (T)(v[r] * inv);
-        *(x4<T>*)((T*)p.out + (long long)row * p.out_row_stride + (long long)head * p.out_head_stride + 4 * lane) = y;
-    }
-    if (p.lse && lane == 0) p.lse[(long long)row * p.lse_row_stride + head] = total == 0.f ? -INFINITY : (top + __log2f(total)) * kLn2;
 }
 
 // ------------------------------------------------------------------ host
 
 constexpr int kMostSplits = 64;
 
-// Splits of the keys: enough workgroups for the chip, but no split below `least_keys` keys of the longest context known.
-int splits_for(long long groups, long long want, long long keys, int least_keys) {
-    const long long s = std::min((want + groups - 1) / groups, (keys + least_keys - 1) / least_keys);
-    return static_cast<int>(std::max(1ll, std::min<long long>(s, kMostSplits)));
-}
-
 Cut cut_of(const PttsPagedAttention& p, int cus) {
     Cut c;
-    const long long G = p.q_heads / p.pages.kv_heads, packed = p.rows * G;
+    const int kvh = p.pages.kv_heads;
+    const long long G = p.q_heads / kvh, packed = p.rows * G;
     const bool is_float = p.q_type == PTTS_TYPE_F32;
     const long long most_rows = p.max_rows > 0 ? std::min(p.max_rows, p.rows) : p.rows;
     long long keys = std::max(1ll, static_cast<long long>(p.table_width) * p.pages.page_size);
@@ -759,22 +805,30 @@ Cut cut_of(const PttsPagedAttention& p, int cus) {
     if (p.window > 0) keys = std::min<long long>(keys, static_cast<long long>(p.window) + p.sinks + most_rows);
     c.few = is_float || p.requests > 1 || most_rows * G <= kFewRows;
     c.chunk = !is_float && most_rows * G > kFewRows;
-    c.few_keys = is_float ? 64 : 128;
-    if (c.few && c.chunk) { c.small = kFewRows; c.few_direct = 1; }
+    if (c.few && c.chunk) c.small = kFewRows;
     c.chunk_tiles = packed / kChunkRows + p.requests;
-    c.few_tiles = c.few_direct ? static_cast<long long>(p.requests) * c.few_direct : packed / kFewRows + p.requests;
+    c.few_tiles = c.small ? p.requests : packed / kFewRows + p.requests;
+    // Splits cost a second launch and a round trip of the rows, so they have to pay: they are made where the tiles alone leave
+    // compute units idle, and no split is shorter than what one workgroup reads in about that time.
+    auto splits = [&](long long groups, long long want, long long least_keys) {
+        const long long s = std::min(want / groups, keys / least_keys);
+        return static_cast<int>(std::max(1ll, std::min<long long>(s, kMostSplits)));
+    };
     if (c.chunk) {
-        const long long groups = std::max(1ll, packed / kChunkRows) * p.pages.kv_heads;
-        c.chunk_splits = splits_for(groups, groups >= cus ? groups : 2ll * cus, keys, 512);
+        const long long groups = std::max(1ll, packed / kChunkRows) * kvh;
+        c.chunk_splits = splits(groups, cus, 1024);
         c.chunk_least = static_cast<int>(std::max(1ll, (keys / kChunkKeys + c.chunk_splits - 1) / c.chunk_splits));
+        c.chunk_parts = static_cast<long long>(p.rows) * p.q_heads;
     }
     if (c.few) {
-        const long long groups = std::max<long long>(p.requests, c.small ? 0 : packed / kFewRows) * p.pages.kv_heads;
-        c.few_splits = splits_for(groups, groups >= 2ll * cus ? groups : 4ll * cus, keys, 2 * c.few_keys);
-        c.few_least = static_cast<int>(std::max(1ll, (keys / c.few_keys + c.few_splits - 1) / c.few_splits));
+        const int step = is_float ? 64 : 128;          // keys of one step of a workgroup
+        const long long groups = std::max<long long>(p.requests, c.small ? 0 : packed / kFewRows) * kvh;
+        c.few_splits = splits(groups, 4ll * cus, (256 << 10) / (2 * p.pages.head_dim * type_size(p.pages.type)));
+        c.few_least = static_cast<int>(std::max(1ll, (keys / step + c.few_splits - 1) / c.few_splits));
+        c.few_parts = c.small ? static_cast<long long>(p.requests) * kvh * kFewRows : static_cast<long long>(p.rows) * p.q_heads;
     }
-    const long long most = std::max(c.chunk_splits, c.few_splits);
-    if (most > 1) c.bytes = most * p.rows * p.q_heads * (p.pages.head_dim + 1ll) * 4;
+    const long long parts = (c.chunk_splits > 1 ? c.chunk_splits * c.chunk_parts : 0) + (c.few_splits > 1 ? c.few_splits * c.few_parts : 0);
+    c.bytes = parts * (p.pages.head_dim + 1ll) * 4;
     return c;
 }
 
@@ -786,9 +840,15 @@ template <typename T, typename C> void launch_few(const AttnArgs& a, unsigned gr
 }
 template <typename T> void launch_chunk(const AttnArgs& a, unsigned grid, hipStream_t s) {
     const int d = a.p.pages.head_dim;
-    if (d <= 64) hipLaunchKernelGGL((attention_chunk_kernel<T, 64>), dim3(grid), dim3(256), 0, s, a);
-    else if (d <= 128) hipLaunchKernelGGL((attention_chunk_kernel<T, 128>), dim3(grid), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((attention_chunk_kernel<T, 256>), dim3(grid), dim3(256), 0, s, a);
+    if (a.few_blocks == 0) {
+        if (d <= 64) hipLaunchKernelGGL((attention_chunk_kernel<T, 64>), dim3(grid), dim3(256), 0, s, a);
+        else if (d <= 128) hipLaunchKernelGGL((attention_chunk_kernel<T, 128>), dim3(grid), dim3(256), 0, s, a);
+        else hipLaunchKernelGGL((attention_chunk_kernel<T, 256>), dim3(grid), dim3(256), 0, s, a);
+    } else {
+        if (d <= 64) hipLaunchKernelGGL((attention_both_kernel<T, 64>), dim3(grid), dim3(256), 0, s, a);
+        else if (d <= 128) hipLaunchKernelGGL((attention_both_kernel<T, 128>), dim3(grid), dim3(256), 0, s, a);
+        else hipLaunchKernelGGL((attention_both_kernel<T, 256>), dim3(grid), dim3(256), 0, s, a);
+    }
 }
 
 unsigned grid_of(long long n) {
@@ -833,37 +893,49 @@ void launch_paged_attention(const PttsPagedAttention& p, int cus, hipStream_t s)
             throw std::runtime_error("paged_attention: a workspace of " + std::to_string(c.bytes) + " bytes is required");
         if (reinterpret_cast<uintptr_t>(p.workspace) % 16) throw std::runtime_error("paged_attention: the workspace must be aligned to 16 bytes");
     }
-    const unsigned chunk_grid = grid_of(c.chunk_tiles * c.chunk_splits * p.pages.kv_heads), few_grid = grid_of(c.few_tiles * c.few_splits * p.pages.kv_heads),
-                   merge_grid = grid_of((static_cast<long long>(p.rows) * p.q_heads + 3) / 4);
+    const long long few_blocks = c.few ? c.few_tiles * c.few_splits * p.pages.kv_heads : 0;
+    const unsigned grid = grid_of(few_blocks + (c.chunk ? c.chunk_tiles * c.chunk_splits * p.pages.kv_heads : 0));
     AttnArgs a;
     a.p = p;
     if (p.window > 1 << 30) a.p.window = 0;          // no context is that long
     a.page = FastDiv::of(static_cast<unsigned>(p.pages.page_size));
     a.group = FastDiv::of(static_cast<unsigned>(p.q_heads / p.pages.kv_heads));
     a.scale2 = p.scale * 1.4426950408889634f;
-    a.part = static_cast<float*>(p.workspace);
-    a.part_lse = a.part + static_cast<long long>(std::max(c.chunk_splits, c.few_splits)) * p.rows * p.q_heads * p.pages.head_dim;
     a.small = c.small;
-    a.merge_few = c.few_splits;
-    a.merge_chunk = c.chunk ? c.chunk_splits : c.few_splits;
+    a.few_blocks = static_cast<unsigned>(few_blocks);
+    a.chunk_tiles = c.chunk_tiles;
+    a.chunk_splits = c.chunk_splits; a.few_splits = c.few_splits;
+    a.chunk_least = c.chunk_least; a.few_least = c.few_least;
+    a.chunk_parts = c.chunk_parts; a.few_parts = c.few_parts;
+    const long long dim = p.pages.head_dim, chunk_rows = c.chunk_splits > 1 ? c.chunk_splits * c.chunk_parts : 0, few_rows = c.few_splits > 1 ? c.few_splits * c.few_parts : 0;
+    a.chunk_part = static_cast<float*>(p.workspace);
+    a.few_part = a.chunk_part + chunk_rows * dim;
+    a.chunk_lse = a.few_part + few_rows * dim;
+    a.few_lse = a.chunk_lse + chunk_rows;
     if (c.chunk) {
-        AttnArgs b = a;
-        b.tiles = c.chunk_tiles; b.splits = c.chunk_splits; b.least = c.chunk_least; b.direct = 0;
-        if (p.q_type == PTTS_TYPE_BF16) launch_chunk<__bf16>(b, chunk_grid, s);
-        else launch_chunk<_Float16>(b, chunk_grid, s);
-    }
-    if (c.few) {
-        AttnArgs b = a;
-        b.tiles = c.few_tiles; b.splits = c.few_splits; b.least = c.few_least; b.direct = c.few_direct;
-        if (p.q_type == PTTS_TYPE_F32 && p.pages.type == PTTS_TYPE_BF16) launch_few<float, __bf16>(b, few_grid, s);
-        else if (p.q_type == PTTS_TYPE_F32) launch_few<float, float>(b, few_grid, s);
-        else if (p.q_type == PTTS_TYPE_BF16) launch_few<__bf16, __bf16>(b, few_grid, s);
-        else launch_few<_Float16, _Float16>(b, few_grid, s);
+        if (p.q_type == PTTS_TYPE_BF16) launch_chunk<__bf16>(a, grid, s);
+        else launch_chunk<_Float16>(a, grid, s);
+    } else if (p.q_type == PTTS_TYPE_F32 && p.pages.type == PTTS_TYPE_BF16) {
+        launch_few<float, __bf16>(a, grid, s);
+    } else if (p.q_type == PTTS_TYPE_F32) {
+        launch_few<float, float>(a, grid, s);
+    } else if (p.q_type == PTTS_TYPE_BF16) {
+        launch_few<__bf16, __bf16>(a, grid, s);
+    } else {
+        launch_few<_Float16, _Float16>(a, grid, s);
     }
     if (c.bytes > 0) {
-        if (p.q_type == PTTS_TYPE_F32) hipLaunchKernelGGL(attention_merge_kernel<float>, dim3(merge_grid), dim3(256), 0, s, a);
-        else if (p.q_type == PTTS_TYPE_BF16) hipLaunchKernelGGL(attention_merge_kernel<__bf16>, dim3(merge_grid), dim3(256), 0, s, a);
-        else hipLaunchKernelGGL(attention_merge_kernel<_Float16>, dim3(merge_grid), dim3(256), 0, s, a);
+        const bool rows_cut = c.chunk ? c.chunk_splits > 1 : true;
+        const unsigned requests = c.small && c.few_splits > 1 ? p.requests : 0;
+        // a request of the few form has at most kFewRows packed rows for each key head, a row q_heads
+        const long long items = std::max<long long>(rows_cut ? p.q_heads : 0, requests ? kFewRows * p.pages.kv_heads : 0) * (p.pages.head_dim / 4);
+        const dim3 merge(grid_of(requests + (rows_cut ? static_cast<long long>(p.rows) : 0)), static_cast<unsigned>((items + 255) / 256));
+        const int splits = c.chunk ? c.chunk_splits : c.few_splits;
+        const float *part = c.chunk ? a.chunk_part : a.few_part, *lse = c.chunk ? a.chunk_lse : a.few_lse;
+        const long long parts = c.chunk ? c.chunk_parts : c.few_parts;
+        if (p.q_type == PTTS_TYPE_F32) hipLaunchKernelGGL(attention_merge_kernel<float>, merge, dim3(256), 0, s, a, requests, splits, part, lse, parts);
+        else if (p.q_type == PTTS_TYPE_BF16) hipLaunchKernelGGL(attention_merge_kernel<__bf16>, merge, dim3(256), 0, s, a, requests, splits, part, lse, parts);
+        else hipLaunchKernelGGL(attention_merge_kernel<_Float16>, merge, dim3(256), 0, s, a, requests, splits, part, lse, parts);
     }
 }
 
