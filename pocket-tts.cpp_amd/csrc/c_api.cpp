@@ -667,8 +667,12 @@ namespace {
 struct OnDevice {
     int before = -1;
     explicit OnDevice(int device) {
-        int n = 0;
-        if (hipGetDeviceCount(&n) != hipSuccess || n == 0) throw std::runtime_error("no HIP device");
+        static std::atomic<int> known{0};
+        int n = known.load();
+        if (n == 0) {
+            if (hipGetDeviceCount(&n) != hipSuccess || n == 0) throw std::runtime_error("no HIP device");
+            known.store(n);
+        }
         if (device < 0 || device >= n) throw std::runtime_error("device " + std::to_string(device) + " of " + std::to_string(n));
         PTTS_HIP(hipGetDevice(&before));
         if (before != device) PTTS_HIP(hipSetDevice(device));

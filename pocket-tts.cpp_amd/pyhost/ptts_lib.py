@@ -153,10 +153,10 @@ def load() -> C.CDLL:
     L.ptts_q8_linear_q.restype = ci; L.ptts_q8_linear_q.argtypes = [vp, f32p, ci, ci, vp, f32p, ci, f32p]
     L.ptts_bf16_linear.restype = ci
     L.ptts_bf16_linear.argtypes = [vp, f32p, ci, ci, f32p, ci, vp, vp, vp, ci, ci, f32p]
-    L.ptts_paged_plan.restype = ci; L.ptts_paged_plan.argtypes = [cp, ci, vp]
-    L.ptts_rotary_append.restype = ci; L.ptts_rotary_append.argtypes = [cp, ci, vp]
-    L.ptts_paged_attention.restype = ci; L.ptts_paged_attention.argtypes = [cp, ci, vp]
-    L.ptts_paged_attention_workspace.restype = C.c_longlong; L.ptts_paged_attention_workspace.argtypes = [cp, ci]
+    L.ptts_paged_plan.restype = ci; L.ptts_paged_plan.argtypes = [vp, ci, vp]          # called through ptts_paged.py
+    L.ptts_rotary_append.restype = ci; L.ptts_rotary_append.argtypes = [vp, ci, vp]
+    L.ptts_paged_attention.restype = ci; L.ptts_paged_attention.argtypes = [vp, ci, vp]
+    L.ptts_paged_attention_workspace.restype = C.c_longlong; L.ptts_paged_attention_workspace.argtypes = [vp, ci]
     L.ptts_rotary_frequencies.restype = ci
     L.ptts_rotary_frequencies.argtypes = [ci, C.c_double, ci, C.c_double, C.c_double, C.c_double, C.c_double, f64p, C.POINTER(C.c_float)]
     L.ptts_weight_bytes.restype = ci; L.ptts_weight_bytes.argtypes = [vp, C.POINTER(C.c_ulonglong)]
