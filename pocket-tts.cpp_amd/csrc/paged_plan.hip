@@ -1,9 +1,13 @@
 // Block tables and slot maps from request lengths, in one launch (formulas: pocket_tts_amd.h, ptts_paged_plan).
 //
-// Every workgroup scans all request lengths itself, 1024 requests at a time, and keeps only the exclusive prefix sums of one
-// such chunk in LDS; it then writes the packed rows of its own slice of the rows and the table entries of its own slice of the
+// Every workgroup scans all request lengths itself, a chunk of requests at a time, and keeps only the exclusive prefix sums of one
+// chunk in LDS; it then writes the packed rows of its own slice of the rows and the table entries of its own slice of the
 // picked pages that fall into the chunk.  One launch and no order between workgroups: nobody reads a table entry that the
 // call writes, because whether a page is old (table) or new (free list) follows from the lengths alone.
+//
+// The sizes are small and the time is a chain of latencies (arguments, lengths, a table entry, the stores), so the chain is kept
+// short: the one old table entry that a request's new rows can fall into is read while the sums are formed, and the head of the
+// free list is read at the start.
 #include <algorithm>
 #include <stdexcept>
 #include <string>
@@ -14,8 +18,7 @@ namespace ptts {
 
 namespace {
 
-constexpr int kChunk = 1024;          // requests scanned at a time (4 per thread)
-constexpr int kSlice = 1024;          // packed rows, and picked pages, of one workgroup
+constexpr int kSlice = 256;           // packed rows, and picked pages, of one workgroup
 
 struct PlanArgs {
     PttsPagedPlan p;
@@ -44,9 +47,11 @@ __device__ __forceinline__ int find_last(const long long* a, int n, long long x)
     return lo;
 }
 
-__global__ __launch_bounds__(256) void plan_kernel(PlanArgs a) {
+// kPer requests a thread and chunk: 1 for up to 256 requests (one round of loads), 4 above (fewer rounds of sums).
+template <int kPer> __global__ __launch_bounds__(256) void plan_kernel(PlanArgs a) {
+    constexpr int kChunk = 256 * kPer;
     __shared__ long long row0[kChunk + 1], pick0[kChunk + 1];
-    __shared__ int cached[kChunk], have[kChunk];
+    __shared__ int cached[kChunk], have[kChunk], tail[kChunk], head[256];
     __shared__ long long part[2][4];
     const PttsPagedPlan& p = a.p;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -56,30 +61,37 @@ __global__ __launch_bounds__(256) void plan_kernel(PlanArgs a) {
     const long long k_lo = (long long)blockIdx.x * kSlice, k_hi = last_wg ? (1ll << 62) : k_lo + kSlice;
     long long rows_before = 0, picks_before = 0, lost_pages = 0, no_page = 0;
     int bad = 0;
+    head[tid] = tid < p.n_free ? p.free_pages[tid] : -1;
+    auto free_page = [&](long long pick) { return pick < 256 ? head[pick] : pick < p.n_free ? p.free_pages[pick] : -1; };
     for (int c0 = 0; c0 < p.requests; c0 += kChunk) {
         const int n = p.requests - c0 < kChunk ? p.requests - c0 : kChunk;
-        const int i0 = 4 * tid;
-        int cach[4], arr[4], hv[4], need[4];
+        const int i0 = kPer * tid;
+        int cach[kPer], arr[kPer], hv[kPer], need[kPer], old[kPer];
         long long rs = 0, ks = 0;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            cach[j] = arr[j] = hv[j] = need[j] = 0;
+        for (int j = 0; j < kPer; ++j) {
+            cach[j] = arr[j] = 0;
             if (i0 + j < n) {
                 cach[j] = p.cached[c0 + i0 + j];
                 arr[j] = p.arriving[c0 + i0 + j];
-                if (cach[j] < 0) { cach[j] = 0; bad = 1; }
-                if (arr[j] < 0) { arr[j] = 0; bad = 1; }
-                if (arr[j] > 0x7fffffff - cach[j]) { arr[j] = 0; bad = 1; }
-                const int end = cach[j] + arr[j];
-                int h = (int)a.page.div(cach[j]), e = (int)a.page.div(end);
-                h += h * ps < cach[j];
-                e += (long long)e * ps < end;
-                if (h > p.table_width) { h = p.table_width; bad = 1; }
-                const int fit = e < p.table_width ? e : p.table_width;
-                lost_pages += e - (fit > h ? fit : h);
-                hv[j] = h;
-                need[j] = fit > h ? fit - h : 0;
             }
+        }
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+            if (cach[j] < 0) { cach[j] = 0; bad = 1; }
+            if (arr[j] < 0) { arr[j] = 0; bad = 1; }
+            if (arr[j] > 0x7fffffff - cach[j]) { arr[j] = 0; bad = 1; }
+            const int end = cach[j] + arr[j], full = (int)a.page.div(cach[j]);
+            int h = full, e = (int)a.page.div(end);
+            h += h * ps < cach[j];
+            e += (long long)e * ps < end;
+            if (h > p.table_width) { h = p.table_width; bad = 1; }
+            // new rows meet one old page at most: the last one, where it is partly filled
+            old[j] = full < h && arr[j] > 0 ? p.block_table[(long long)(c0 + i0 + j) * p.table_stride + full] : -1;
+            const int fit = e < p.table_width ? e : p.table_width;
+            lost_pages += e - (fit > h ? fit : h);
+            hv[j] = h;
+            need[j] = fit > h ? fit - h : 0;
             rs += arr[j];
             ks += need[j];
         }
@@ -94,11 +106,12 @@ __global__ __launch_bounds__(256) void plan_kernel(PlanArgs a) {
             picks_before += part[1][w];
         }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < kPer; ++j) {
             row0[i0 + j] = r;
             pick0[i0 + j] = k;
             cached[i0 + j] = cach[j];
             have[i0 + j] = hv[j];
+            tail[i0 + j] = old[j];
             if (i0 + j < n && (unsigned)(c0 / kChunk) % gridDim.x == blockIdx.x) {
                 p.cu_rows[c0 + i0 + j] = (int)(r < 0x7fffffff ? r : 0x7fffffff);
                 p.kv_len[c0 + i0 + j] = cach[j] + arr[j];
@@ -112,33 +125,22 @@ __global__ __launch_bounds__(256) void plan_kernel(PlanArgs a) {
         }
         if (tid == 255) { row0[kChunk] = r; pick0[kChunk] = k; }
         __syncthreads();
-        // packed rows of this workgroup's slice, four in a row per thread
-        const long long ra = r_lo > row0[0] ? r_lo : row0[0], rb = r_hi < row0[kChunk] ? r_hi : row0[kChunk];
-        for (long long q = ra + 4 * tid; q < rb; q += 4 * 256) {
-            int i = find_last(row0, kChunk, q);
-            for (int j = 0; j < 4 && q + j < rb; ++j) {
-                while (q + j >= row0[i + 1]) ++i;
-                const int pos = cached[i] + (int)(q + j - row0[i]);
-                const int pg = (int)a.page.div(pos);
-                int id = -1;
-                if (pg < p.table_width) {
-                    if (pg < have[i]) id = p.block_table[(long long)(c0 + i) * p.table_stride + pg];
-                    else {
-                        const long long pick = pick0[i] + pg - have[i];
-                        if (pick < p.n_free) id = p.free_pages[pick];
-                    }
-                }
-                long long slot = id < 0 ? -1 : (long long)id * ps + (pos - pg * ps);
-                if (slot > 0x7fffffff) { slot = -1; bad |= 2; }
-                p.slot_map[q + j] = (int)slot;
-                p.positions[q + j] = pos;
-            }
+        // packed rows of this workgroup's slice
+        const long long ra = r_lo > row0[0] ? r_lo : row0[0], rb = r_hi < row0[n] ? r_hi : row0[n];
+        for (long long q = ra + tid; q < rb; q += 256) {
+            const int i = find_last(row0, n, q), pos = cached[i] + (int)(q - row0[i]), pg = (int)a.page.div(pos);
+            int id = -1;
+            if (pg < p.table_width) id = pg < have[i] ? tail[i] : free_page(pick0[i] + pg - have[i]);
+            long long slot = id < 0 ? -1 : (long long)id * ps + (pos - pg * ps);
+            if (slot > 0x7fffffff) { slot = -1; bad |= 2; }
+            p.slot_map[q] = (int)slot;
+            p.positions[q] = pos;
         }
         // table entries of this workgroup's slice of the picked pages
-        const long long ka = k_lo > pick0[0] ? k_lo : pick0[0], kb = k_hi < pick0[kChunk] ? k_hi : pick0[kChunk];
+        const long long ka = k_lo > pick0[0] ? k_lo : pick0[0], kb = k_hi < pick0[n] ? k_hi : pick0[n];
         for (long long q = ka + tid; q < kb; q += 256) {
-            const int i = find_last(pick0, kChunk, q);
-            p.block_table[(long long)(c0 + i) * p.table_stride + have[i] + (int)(q - pick0[i])] = q < p.n_free ? p.free_pages[q] : -1;
+            const int i = find_last(pick0, n, q);
+            p.block_table[(long long)(c0 + i) * p.table_stride + have[i] + (int)(q - pick0[i])] = free_page(q);
         }
     }
     // totals, the same in every workgroup
@@ -185,7 +187,9 @@ void launch_paged_plan(const PttsPagedPlan& p, hipStream_t s) {
     const long long most = static_cast<long long>(p.rows) / p.page_size + p.requests;
     a.picks = most < p.n_free ? most : p.n_free;
     const long long slices = std::max<long long>((p.rows + kSlice - 1) / kSlice, (a.picks + kSlice - 1) / kSlice);
-    hipLaunchKernelGGL(plan_kernel, dim3(static_cast<unsigned>(std::max<long long>(slices, 1))), dim3(256), 0, s, a);
+    const dim3 grid(static_cast<unsigned>(std::max<long long>(slices, 1)));
+    if (p.requests <= 256) hipLaunchKernelGGL(plan_kernel<1>, grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL(plan_kernel<4>, grid, dim3(256), 0, s, a);
 }
 
 }  // namespace ptts
