@@ -217,12 +217,16 @@ template <int DH> __device__ __forceinline__ int key_swizzle(int row) { return D
 template <int DH> __device__ __forceinline__ int value_swizzle(int row) { return DH >= 128 ? (row & 3) << 2 : ((row >> 1) & 1) << 2; }
 
 template <typename T, int DH> struct ChunkLds {
-    T k[kChunkKeys * DH], v[kChunkKeys * DH];
+    T k[2][kChunkKeys * DH], v[2][kChunkKeys * DH];      // one block is read while the next arrives
 };
+
+// 16 bytes a lane from memory to LDS: lane l's land at `to` + 16 l
+__device__ __forceinline__ void copy16(const void* from, void* to) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) unsigned*)from, (__attribute__((address_space(3))) unsigned*)to, 16, 0, 0);
+}
 
 template <typename T, int DH> __device__ __forceinline__ void chunk_body(const AttnArgs& a, unsigned block, ChunkLds<T, DH>& lds) {
     constexpr int kUnits = DH / 8, kPassRows = 256 / kUnits, kPasses = kChunkKeys / kPassRows, KS = DH / 16, NT = DH / 32;
-    T *const Ks = lds.k, *const Vs = lds.v;
     const PttsPagedAttention& p = a.p;
     const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);   // matrix instructions ignore the lane mask: every branch around one is scalar
@@ -257,28 +261,32 @@ template <typename T, int DH> __device__ __forceinline__ void chunk_body(const A
 
     const int* table = p.block_table + (long long)t.i * p.table_stride;
     const int unit = tid % kUnits, sr = tid / kUnits;
-    const bool unit_live = unit * 8 < dim;
-    uint4 kreg[kPasses], vreg[kPasses];
-#pragma unroll
-    for (int i = 0; i < kPasses; ++i) kreg[i] = vreg[i] = make_uint4(0, 0, 0, 0);    // units behind the head's values stay zero
+    const int place = (wave * (kPassRows / 4)) * DH;       // of the wave's rows in a pass
     int bad = t.bad, id = kUnseen;
-    unsigned long long holes = 0;           // keys of the block on its way that were not read
+    unsigned long long holes = 0;           // keys of the block on its way that are not read
+    if (dim < DH) {                         // units behind the head's values stay zero
+        for (int i = tid; i < (int)(sizeof(lds) / 16); i += 256) reinterpret_cast<uint4*>(&lds)[i] = make_uint4(0, 0, 0, 0);
+        __syncthreads();
+    }
     // Lane l of every wave looks up key l of a block, one block before its rows are read; the threads that copy the row take its
     // place from there.
     auto look_up = [&](int u) { id = page_of(a, t, table, list.block(u) * kChunkKeys + lane); };
-    auto load = [&](int u) {
+    auto load = [&](int u, int into) {
         bool ok;
         const long long mine = row_at(a, id, list.block(u) * kChunkKeys + lane, kvh, bad, ok);
         holes = __ballot(!ok);
         long long at[kPasses];
 #pragma unroll
-        for (int i = 0; i < kPasses; ++i) at[i] = __shfl(mine, sr + kPassRows * i, 64) + unit * 8;
-        if (unit_live) {
+        for (int i = 0; i < kPasses; ++i) at[i] = __shfl(mine, sr + kPassRows * i, 64);
 #pragma unroll
-            for (int i = 0; i < kPasses; ++i) {
-                kreg[i] = *(const uint4*)((const T*)p.pages.k + at[i]);
-                vreg[i] = *(const uint4*)((const T*)p.pages.v + at[i]);
-            }
+        for (int i = 0; i < kPasses; ++i) {
+            const int c = (unit ^ key_swizzle<DH>(sr + kPassRows * i)) * 8;      // the unit that lies at this lane's place
+            if (DH == dim || c < dim) copy16((const T*)p.pages.k + at[i] + c, lds.k[into] + place + i * kPassRows * DH);
+        }
+#pragma unroll
+        for (int i = 0; i < kPasses; ++i) {
+            const int c = (unit ^ value_swizzle<DH>(sr + kPassRows * i)) * 8;
+            if (DH == dim || c < dim) copy16((const T*)p.pages.v + at[i] + c, lds.v[into] + place + i * kPassRows * DH);
         }
     };
 
@@ -292,11 +300,12 @@ template <typename T, int DH> __device__ __forceinline__ void chunk_body(const A
     const int vrow = 4 * h + ((lane & 15) >> 2);
     const int vunit = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), vx = value_swizzle<DH>(vrow);
     int kbase = col * DH * 2 + ((key_swizzle<DH>(col) ^ h) << 4), vbase = vrow * DH * 2 + 8 * (lane & 1);    // bytes
+    int now = 0;
     auto key_frag = [&](int b, int ks) {    // rows 32 b + col, head values 16 ks + 8 h ..: the swizzle is a part of kbase
-        return *(const x8<T>*)((const char*)Ks + (kbase ^ (ks << 5)) + b * 32 * DH * 2);
+        return *(const x8<T>*)((const char*)lds.k[now] + (kbase ^ (ks << 5)) + b * 32 * DH * 2);
     };
     auto value = [&](int n, int s) {        // V^T of 32 head values from 32 n and keys 16 s ..: keys 4 h + 0..3 and 8 + 4 h + 0..3
-        const char* at = (const char*)Vs + vbase + (((4 * n + vunit) ^ vx) << 4) + 16 * s * DH * 2;
+        const char* at = (const char*)lds.v[now] + vbase + (((4 * n + vunit) ^ vx) << 4) + 16 * s * DH * 2;
         union { s16x4 w[2]; x8<T> v; } u;
         u.w[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at);
         u.w[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(at + 8 * DH * 2));
@@ -306,31 +315,30 @@ template <typename T, int DH> __device__ __forceinline__ void chunk_body(const A
     unsigned kept = ~0u;
     if (u0 < u1) {
         look_up(u0);
-        load(u0);
+        load(u0, 0);
         if (u0 + 1 < u1) look_up(u0 + 1);
     }
     for (int u = u0; u < u1; ++u) {
         const int k0 = list.block(u) * kChunkKeys, k1 = k0 + kChunkKeys - 1;
         const bool border = !all_seen(p, k0, k1, t.p0, t.p1);       // some row of the tile does not see the block whole
-        if (holes) {
+        now = (u - u0) & 1;
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");            // what this wave copied has landed
+        if (holes || border) {
 #pragma unroll
-            for (int i = 0; i < kPasses; ++i)
-                if ((holes >> (sr + kPassRows * i)) & 1) kreg[i] = vreg[i] = make_uint4(0, 0, 0, 0);
+            for (int i = 0; i < kPasses; ++i) {
+                uint4* kp = reinterpret_cast<uint4*>(lds.k[now] + place + i * kPassRows * DH) + lane;
+                uint4* vp = reinterpret_cast<uint4*>(lds.v[now] + place + i * kPassRows * DH) + lane;
+                if ((holes >> (sr + kPassRows * i)) & 1) { *kp = make_uint4(0, 0, 0, 0); *vp = make_uint4(0, 0, 0, 0); }
+                else if (border) {
+                    uint4 x = *vp;
+                    clean<T>(reinterpret_cast<unsigned(&)[4]>(x), kept);
+                    *vp = x;
+                }
+            }
         }
-        if (border) {
-#pragma unroll
-            for (int i = 0; i < kPasses; ++i) clean<T>(reinterpret_cast<unsigned(&)[4]>(vreg[i]), kept);
-        }
-        __syncthreads();                    // the previous block is consumed
-#pragma unroll
-        for (int i = 0; i < kPasses; ++i) {
-            const int r = sr + kPassRows * i;
-            *(uint4*)(Ks + r * DH + (unit ^ key_swizzle<DH>(r)) * 8) = kreg[i];
-            *(uint4*)(Vs + r * DH + (unit ^ value_swizzle<DH>(r)) * 8) = vreg[i];
-        }
-        __syncthreads();
+        __syncthreads();                    // the block is whole, and the one before is consumed
         if (u + 1 < u1) {
-            load(u + 1);
+            load(u + 1, now ^ 1);
             if (u + 2 < u1) look_up(u + 2);
         }
         if (idle || (border && none_seen(p, k0, k1, pw0, pw1))) continue;
@@ -463,15 +471,18 @@ template <typename T, typename C, int DH> struct Step {
 };
 
 template <int DH> struct FewLds {
-    float joined[4][kFewRows][DH + 4];      // +4: the waves' columns of one row do not meet in one bank
+    union {
+        long long places[4][32];                   // where the keys of a step lie: the step at work, the next and the one after
+        float joined[kFewRows][DH + 4];            // +4: the waves' columns of one row do not meet in one bank
+    } of[4];                                       // one for each wave
     float tops[4][kFewRows], sums[4][kFewRows];
 };
 
-template <typename T, typename C, int DH> __device__ __forceinline__ void few_body(const AttnArgs& a, unsigned block, FewLds<DH>& lds) {
+// kFull: the head fills DH, so that no lane's values lie behind it.
+template <typename T, typename C, int DH, bool kFull> __device__ __forceinline__ void few_body(const AttnArgs& a, unsigned block, FewLds<DH>& lds) {
     using S = Step<T, C, DH>;
     constexpr int NA = S::NA, CPL = S::CPL, KS = S::KS, KW = S::KW, VW = S::VW, VN = S::VN, kWaveKeys = 16 * NA, kKeys = 4 * kWaveKeys;
     constexpr bool kFloat = S::kFloat;
-    auto &joined = lds.joined;
     auto &tops = lds.tops, &sums = lds.sums;
     const PttsPagedAttention& p = a.p;
     const int tid = threadIdx.x, lane = tid & 63, li = lane & 15, g = lane >> 4;
@@ -498,34 +509,41 @@ template <typename T, typename C, int DH> __device__ __forceinline__ void few_bo
     }
 
     const int* table = p.block_table + (long long)t.i * p.table_stride;
-    int bad = t.bad, ids[NA];
-    auto look_up = [&](int u) {
-        const int k0 = list.block(u) * kKeys + wave * kWaveKeys;
-#pragma unroll
-        for (int b = 0; b < NA; ++b) ids[b] = page_of(a, t, table, k0 + 16 * b + li);
+    int bad = t.bad;
+    // Every step issues the same reads in the same order (page ids three steps ahead, rows one step ahead), whatever it will see of
+    // them: waits count reads, and a branch around one would make the compiler wait for all.  Keys that are not read after
+    // all are taken from the pool's first row and replaced by zeros when their step is at work.
+    auto& mine = lds.of[wave];
+    const int kk = lane % kWaveKeys;
+    auto key_of = [&](int u, int k) { return list.block(u) * kKeys + wave * kWaveKeys + k; };
+    auto fetch = [&](int u) { return table[a.page.div(min(key_of(min(u, u1 - 1), kk), t.p1))]; };
+    auto settle = [&](int u, int id) {      // returns the keys of the step that are read, a bit each
+        u = min(u, u1 - 1);
+        const int key = key_of(u, kk);
+        bool ok;
+        const long long at = row_at(a, key <= t.p1 && (key >= t.low || key < p.sinks) ? id : kUnseen, min(key, t.p1), kvh, bad, ok);
+        mine.places[u & 3][kk] = at;
+        __builtin_amdgcn_wave_barrier();
+        return (unsigned)__ballot(ok) | (kWaveKeys < 32 ? ~0u << (kWaveKeys & 31) : 0u);
     };
     auto load = [&](int u, S& x) {
-        const int k0 = list.block(u) * kKeys + wave * kWaveKeys;
+        const long long* at = mine.places[min(u, u1 - 1) & 3];
 #pragma unroll
         for (int b = 0; b < NA; ++b) {
-            bool ok;
-            const long long at = row_at(a, ids[b], k0 + 16 * b + li, kvh, bad, ok);
-            const unsigned there = (unsigned)__ballot(ok);             // keys li of lanes 0 .. 15
+            const C* k = (const C*)p.pages.k + at[16 * b + li];
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
-                const typename S::kvec zero = {};
                 const int d = 4 * KW * ks + KW * g;
-                x.k[b][ks] = ok && d < dim ? *(const typename S::kvec*)((const C*)p.pages.k + at + d) : zero;
+                x.k[b][ks] = *(const typename S::kvec*)(k + (kFull || d < dim ? d : 0));
             }
+        }
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const long long from = __shfl(at, 4 * g + r, 64);
+        for (int r = 0; r < 4 * NA; ++r) {
+            const C* v = (const C*)p.pages.v + at[16 * (r >> 2) + 4 * g + (r & 3)];
 #pragma unroll
-                for (int n = 0; n < VN; ++n) {
-                    const typename S::vvec zero = {};
-                    const int d = CPL * li + VW * n;
-                    x.v[4 * b + r][n] = ((there >> (4 * g + r)) & 1) && d < dim ? *(const typename S::vvec*)((const C*)p.pages.v + from + d) : zero;
-                }
+            for (int n = 0; n < VN; ++n) {
+                const int d = CPL * li + VW * n;
+                x.v[r][n] = *(const typename S::vvec*)(v + (kFull || d < dim ? d : 0));      // what lies behind the head is not stored
             }
         }
     };
@@ -536,9 +554,28 @@ template <typename T, typename C, int DH> __device__ __forceinline__ void few_bo
     float top = -INFINITY, sum = 0.f;
 
     unsigned kept = ~0u;
-    auto work = [&](int u, S& x) {
+    auto work = [&](int u, S& x, unsigned there) {
         const int k0 = list.block(u) * kKeys + wave * kWaveKeys, k1 = k0 + kWaveKeys - 1;
         if (none_seen(p, k0, k1, t.p0, t.p1)) return;
+        if constexpr (!kFull) {
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks)
+                if (4 * KW * ks + KW * g >= dim)
+#pragma unroll
+                    for (int b = 0; b < NA; ++b) x.k[b][ks] = typename S::kvec{};
+        }
+        if (there != ~0u) {
+#pragma unroll
+            for (int b = 0; b < NA; ++b)
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks)
+                    if (!((there >> (16 * b + li)) & 1)) x.k[b][ks] = typename S::kvec{};
+#pragma unroll
+            for (int r = 0; r < 4 * NA; ++r)
+#pragma unroll
+                for (int n = 0; n < VN; ++n)
+                    if (!((there >> (16 * (r >> 2) + 4 * g + (r & 3))) & 1)) x.v[r][n] = typename S::vvec{};
+        }
         f32x4 s[NA];
 #pragma unroll
         for (int b = 0; b < NA; ++b) {
@@ -616,35 +653,33 @@ template <typename T, typename C, int DH> __device__ __forceinline__ void few_bo
         }
     };
 
-    S one, two;
     if (u0 < u1) {
-        look_up(u0);
+        S one, two;
+        const int first = fetch(u0), second = fetch(u0 + 1);
+        int id = fetch(u0 + 2);
+        unsigned now = settle(u0, first), next = settle(u0 + 1, second);
         load(u0, one);
-        if (u0 + 1 < u1) look_up(u0 + 1);
-    }
-    for (int u = u0; u < u1; u += 2) {
-        if (u + 1 < u1) {
+        for (int u = u0; u < u1; u += 2) {
+            int after = fetch(u + 3);
             load(u + 1, two);
-            if (u + 2 < u1) look_up(u + 2);
-        }
-        work(u, one);
-        if (u + 1 < u1) {
-            if (u + 2 < u1) {
-                load(u + 2, one);
-                if (u + 3 < u1) look_up(u + 3);
-            }
-            work(u + 1, two);
+            unsigned then = settle(u + 2, id);
+            work(u, one, now);
+            id = fetch(u + 4);
+            load(u + 2, one);
+            now = then;
+            then = settle(u + 3, after);
+            if (u + 1 < u1) work(u + 1, two, next);
+            next = then;
         }
     }
     if (__any(kept != ~0u)) {
         for (int u = u0; u < u1; ++u) {
             const int k0 = list.block(u) * kKeys + wave * kWaveKeys;
             if (all_seen(p, k0, k0 + kWaveKeys - 1, t.p0, t.p1) || none_seen(p, k0, k0 + kWaveKeys - 1, t.p0, t.p1)) continue;
-            look_up(u);
 #pragma unroll
             for (int b = 0; b < NA; ++b) {
                 bool ok;
-                const long long mine = row_at(a, ids[b], k0 + 16 * b + li, kvh, bad, ok);
+                const long long mine = row_at(a, page_of(a, t, table, k0 + 16 * b + li), k0 + 16 * b + li, kvh, bad, ok);
                 const unsigned there = (unsigned)__ballot(ok);
 #pragma unroll 1
                 for (int j = 0; j < 16; ++j) {
@@ -653,9 +688,13 @@ template <typename T, typename C, int DH> __device__ __forceinline__ void few_bo
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
 #pragma unroll
-                        for (int n = 0; n < CPL; ++n)
-                            if (CPL * (4 * g + r) + n < dim)
-                                o[n][r] = add_not_finite(o[n][r], (float)((const C*)p.pages.v)[at + CPL * (4 * g + r) + n]);
+                        for (int n = 0; n < VN; ++n) {
+                            const int d = CPL * (4 * g + r) + VW * n;
+                            if (d >= dim) continue;
+                            const typename S::vvec v = *(const typename S::vvec*)((const C*)p.pages.v + at + d);
+#pragma unroll
+                            for (int c = 0; c < VW; ++c) o[VW * n + c][r] = add_not_finite(o[VW * n + c][r], (float)v[c]);
+                        }
                 }
             }
         }
@@ -669,14 +708,14 @@ template <typename T, typename C, int DH> __device__ __forceinline__ void few_bo
     float all = -INFINITY;
 #pragma unroll
     for (int w = 0; w < 4; ++w) all = fmaxf(all, tops[w][li]);
-    const float mine = top == -INFINITY ? 0.f : exp2_of(top - all);
+    const float weight = top == -INFINITY ? 0.f : exp2_of(top - all);
     const int n_live = t.m1 - t.m0;
     if (li < n_live) {
 #pragma unroll
         for (int r = 0; r < 4; ++r)
 #pragma unroll
             for (int n = 0; n < CPL; n += 4)
-                *(f32x4*)&joined[wave][li][CPL * (4 * g + r) + n] = f32x4{o[n][r], o[n + 1][r], o[n + 2][r], o[n + 3][r]} * mine;
+                *(f32x4*)&mine.joined[li][CPL * (4 * g + r) + n] = f32x4{o[n][r], o[n + 1][r], o[n + 2][r], o[n + 3][r]} * weight;
     }
     __syncthreads();
     const int quads = dim / 4;
@@ -687,9 +726,9 @@ template <typename T, typename C, int DH> __device__ __forceinline__ void few_bo
         for (int w = 0; w < 4; ++w) big = fmaxf(big, tops[w][q]);
 #pragma unroll
         for (int w = 0; w < 4; ++w) total += tops[w][q] == -INFINITY ? 0.f : sums[w][q] * exp2_of(tops[w][q] - big);
-        f32x4 v = *(f32x4*)&joined[0][q][d];
+        f32x4 v = *(f32x4*)&lds.of[0].joined[q][d];
 #pragma unroll
-        for (int w = 1; w < 4; ++w) v += *(f32x4*)&joined[w][q][d];
+        for (int w = 1; w < 4; ++w) v += *(f32x4*)&lds.of[w].joined[q][d];
         const float inv = total == 0.f ? 0.f : 1.0f / total, lse2 = total == 0.f ? -INFINITY : big + __log2f(total);
         const int mq = t.m0 + q, tq = a.group.div(mq), hq = kvh * G + mq - tq * G;
         const long long rq = t.row0 + tq;
@@ -708,22 +747,22 @@ template <typename T, typename C, int DH> __device__ __forceinline__ void few_bo
 }
 
 // The forms' entries.  A launch of the few form alone does not carry the chunk form's registers and LDS.
-template <typename T, typename C, int DH> __global__ __launch_bounds__(256, DH == 256 ? 1 : 2) void attention_few_kernel(AttnArgs a) {
+template <typename T, typename C, int DH, bool kFull> __global__ __launch_bounds__(256, DH == 256 ? 1 : DH == 128 ? 2 : 3) void attention_few_kernel(AttnArgs a) {
     __shared__ __attribute__((aligned(16))) FewLds<DH> lds;
-    few_body<T, C, DH>(a, blockIdx.x, lds);
+    few_body<T, C, DH, kFull>(a, blockIdx.x, lds);
 }
 // Three workgroups per CU where the head fits (170 registers), else two.
 template <typename T, int DH> __global__ __launch_bounds__(256, DH == 256 ? 1 : DH == 128 ? 2 : 3) void attention_chunk_kernel(AttnArgs a) {
     __shared__ __attribute__((aligned(16))) ChunkLds<T, DH> lds;
     chunk_body<T, DH>(a, blockIdx.x, lds);
 }
-template <typename T, int DH> __global__ __launch_bounds__(256, DH == 256 ? 1 : DH == 128 ? 2 : 3) void attention_both_kernel(AttnArgs a) {
+template <typename T, int DH, bool kFull> __global__ __launch_bounds__(256, DH == 256 ? 1 : DH == 128 ? 2 : 3) void attention_both_kernel(AttnArgs a) {
     __shared__ __attribute__((aligned(16))) union Lds {
         ChunkLds<T, DH> chunk;
         FewLds<DH> few;
         __device__ Lds() {}
     } lds;
-    if (blockIdx.x < a.few_blocks) few_body<T, T, DH>(a, blockIdx.x, lds.few);
+    if (blockIdx.x < a.few_blocks) few_body<T, T, DH, kFull>(a, blockIdx.x, lds.few);
     else chunk_body<T, DH>(a, blockIdx.x - a.few_blocks, lds.chunk);
 }
 
@@ -733,16 +772,31 @@ template <typename T, int DH> __global__ __launch_bounds__(256, DH == 256 ? 1 : 
 template <typename T>
 __device__ __forceinline__ void merge_one(const PttsPagedAttention& p, const float* part, const float* lse, long long stride, int splits, long long at, long long row,
                                           int head, int d) {
-    float top = -INFINITY;
-    for (int s = 0; s < splits; ++s) top = fmaxf(top, lse[s * stride + at]);
-    float total = 0.f;
+    // four splits at a time, so that their reads are on their way together; a split that saw nothing wrote no values
+    float top = -INFINITY, total = 0.f;
     f32x4 v = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < splits; ++s) {
-        const float l = lse[s * stride + at];
-        if (l == -INFINITY) continue;                 // nothing seen there, and no values written
-        const float w = exp2_of(l - top);
-        total += w;
-        v += *(const f32x4*)(part + (s * stride + at) * p.pages.head_dim + d) * w;
+    for (int s = 0; s < splits; s += 4) {
+        float l[4];
+        f32x4 x[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const long long from = min(s + j, splits - 1) * stride + at;
+            l[j] = s + j < splits ? lse[from] : -INFINITY;
+            x[j] = *(const f32x4*)(part + from * p.pages.head_dim + d);
+        }
+        const float next = fmaxf(fmaxf(top, fmaxf(l[0], l[1])), fmaxf(l[2], l[3]));
+        if (next == -INFINITY) continue;
+        const float fade = exp2_of(top - next);
+        top = next;
+        total *= fade;
+        v *= fade;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (l[j] != -INFINITY) {
+                const float w = exp2_of(l[j] - top);
+                total += w;
+                v += x[j] * w;
+            }
     }
     const float inv = total == 0.f ? 0.f : 1.0f / total;
     x4<T> y;
@@ -823,7 +877,8 @@ Cut cut_of(const PttsPagedAttention& p, int cus) {
     if (c.few) {
         const int step = is_float ? 64 : 128;          // keys of one step of a workgroup
         const long long groups = std::max<long long>(p.requests, c.small ? 0 : packed / kFewRows) * kvh;
-        c.few_splits = splits(groups, 4ll * cus, (256 << 10) / (2 * p.pages.head_dim * type_size(p.pages.type)));
+        const long long resident = p.pages.head_dim <= 64 ? 3 : p.pages.head_dim <= 128 ? 2 : 1;       // workgroups of a compute unit
+        c.few_splits = splits(groups, resident * cus, (256 << 10) / (2 * p.pages.head_dim * type_size(p.pages.type)));
         c.few_least = static_cast<int>(std::max(1ll, (keys / step + c.few_splits - 1) / c.few_splits));
         c.few_parts = c.small ? static_cast<long long>(p.requests) * kvh * kFewRows : static_cast<long long>(p.rows) * p.q_heads;
     }
@@ -832,23 +887,26 @@ Cut cut_of(const PttsPagedAttention& p, int cus) {
     return c;
 }
 
+template <typename T, typename C, int DH> void launch_few_of(const AttnArgs& a, unsigned grid, hipStream_t s) {
+    if (a.p.pages.head_dim == DH) hipLaunchKernelGGL((attention_few_kernel<T, C, DH, true>), dim3(grid), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((attention_few_kernel<T, C, DH, false>), dim3(grid), dim3(256), 0, s, a);
+}
 template <typename T, typename C> void launch_few(const AttnArgs& a, unsigned grid, hipStream_t s) {
     const int d = a.p.pages.head_dim;
-    if (d <= 64) hipLaunchKernelGGL((attention_few_kernel<T, C, 64>), dim3(grid), dim3(256), 0, s, a);
-    else if (d <= 128) hipLaunchKernelGGL((attention_few_kernel<T, C, 128>), dim3(grid), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((attention_few_kernel<T, C, 256>), dim3(grid), dim3(256), 0, s, a);
+    if (d <= 64) launch_few_of<T, C, 64>(a, grid, s);
+    else if (d <= 128) launch_few_of<T, C, 128>(a, grid, s);
+    else launch_few_of<T, C, 256>(a, grid, s);
+}
+template <typename T, int DH> void launch_chunk_of(const AttnArgs& a, unsigned grid, hipStream_t s) {
+    if (a.few_blocks == 0) hipLaunchKernelGGL((attention_chunk_kernel<T, DH>), dim3(grid), dim3(256), 0, s, a);
+    else if (a.p.pages.head_dim == DH) hipLaunchKernelGGL((attention_both_kernel<T, DH, true>), dim3(grid), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((attention_both_kernel<T, DH, false>), dim3(grid), dim3(256), 0, s, a);
 }
 template <typename T> void launch_chunk(const AttnArgs& a, unsigned grid, hipStream_t s) {
     const int d = a.p.pages.head_dim;
-    if (a.few_blocks == 0) {
-        if (d <= 64) hipLaunchKernelGGL((attention_chunk_kernel<T, 64>), dim3(grid), dim3(256), 0, s, a);
-        else if (d <= 128) hipLaunchKernelGGL((attention_chunk_kernel<T, 128>), dim3(grid), dim3(256), 0, s, a);
-        else hipLaunchKernelGGL((attention_chunk_kernel<T, 256>), dim3(grid), dim3(256), 0, s, a);
-    } else {
-        if (d <= 64) hipLaunchKernelGGL((attention_both_kernel<T, 64>), dim3(grid), dim3(256), 0, s, a);
-        else if (d <= 128) hipLaunchKernelGGL((attention_both_kernel<T, 128>), dim3(grid), dim3(256), 0, s, a);
-        else hipLaunchKernelGGL((attention_both_kernel<T, 256>), dim3(grid), dim3(256), 0, s, a);
-    }
+    if (d <= 64) launch_chunk_of<T, 64>(a, grid, s);
+    else if (d <= 128) launch_chunk_of<T, 128>(a, grid, s);
+    else launch_chunk_of<T, 256>(a, grid, s);
 }
 
 unsigned grid_of(long long n) {
