@@ -103,6 +103,17 @@ POCKET_TTS_API void* ptts_state_new(PocketTTSHandle handle, int batch);
 POCKET_TTS_API void ptts_state_free(PocketTTSHandle handle, void* state);
 POCKET_TTS_API int ptts_state_reset(PocketTTSHandle handle, void* state);
 
+/* The same with the LM's keys and values in a pool of `pages` pages of page_size rows that the slots share, up to max_context rows
+ * each (ptts_paged_plan, ptts_rotary_append and ptts_paged_attention below run inside).  window > 0: a row sees the last `window` rows
+ * and the first `sinks` ones, and pages behind the window return to the pool.  ptts_lm_prefill may be called repeatedly (a prompt
+ * in chunks); a call that needs more pages than are free fails and changes nothing.  No counterpart in the reference. */
+POCKET_TTS_API void* ptts_state_new_paged(PocketTTSHandle handle, int batch, int pages, int page_size, int max_context, int window, int sinks);
+/* Slot to_slot of a paged state begins anew with the first `rows` rows of from_slot (one voice for many utterances): whole pages
+ * are shared, the rest is copied. */
+POCKET_TTS_API int ptts_state_share(PocketTTSHandle handle, void* state, int from_slot, int to_slot, int rows);
+/* Free pages of a paged state's pool. */
+POCKET_TTS_API int ptts_state_free_pages(PocketTTSHandle handle, void* state);
+
 /* flow_lm_main, prefill shape: sequence empty, text_embeddings = emb[rows][d_model] for one utterance
  * (src/pocket_tts.cpp:572,575). */
 POCKET_TTS_API int ptts_lm_prefill(PocketTTSHandle handle, void* state, int slot, const float* emb, int rows);

@@ -419,6 +419,35 @@ POCKET_TTS_API void* ptts_state_new(PocketTTSHandle handle, int batch) {
     }
 }
 
+POCKET_TTS_API void* ptts_state_new_paged(PocketTTSHandle handle, int batch, int pages, int page_size, int max_context, int window, int sinks) {
+    if (!handle || batch <= 0) { set_error("Invalid parameters"); return nullptr; }
+    try {
+        ptts::PagedOptions o;
+        o.pages = pages; o.page_size = page_size; o.max_context = max_context; o.window = window; o.sinks = sinks;
+        return tts_of(handle)->engine().batch_new_paged(batch, o);
+    } catch (const std::exception& e) {
+        set_error(std::string("state_new_paged: ") + e.what());
+        return nullptr;
+    }
+}
+
+POCKET_TTS_API int ptts_state_share(PocketTTSHandle handle, void* state, int from_slot, int to_slot, int rows) {
+    if (!handle || !state) { set_error("Invalid parameters"); return -1; }
+    return guarded("state_share: ", [&] {
+        tts_of(handle)->engine().op_state_share(static_cast<ptts::Batch*>(state), from_slot, to_slot, rows);
+        return 0;
+    });
+}
+
+POCKET_TTS_API int ptts_state_free_pages(PocketTTSHandle handle, void* state) {
+    if (!handle || !state) { set_error("Invalid parameters"); return -1; }
+    return guarded("state_free_pages: ", [&] {
+        const auto* b = static_cast<ptts::Batch*>(state);
+        if (!b->paged) throw std::runtime_error("the state was not created with pages");
+        return b->paged->free_count();
+    });
+}
+
 POCKET_TTS_API void ptts_state_free(PocketTTSHandle handle, void* state) {
     if (handle && state) tts_of(handle)->engine().batch_free(static_cast<ptts::Batch*>(state));
 }

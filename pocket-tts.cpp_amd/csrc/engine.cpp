@@ -535,7 +535,7 @@ void Model::build_rope_tables(int lm_len, int mimi_len) {
 
 static constexpr int kDecChunk = 15;  // frames per decoder call, /root/reference/src/pocket_tts.cpp:461
 
-Batch::Batch(Engine& e, int B_, bool lm_only_) : B(B_), Bw(B_), lm_only(lm_only_) {
+Batch::Batch(Engine& e, int B_, bool lm_only_, const PagedOptions* pages) : B(B_), Bw(B_), lm_only(lm_only_) {
     st = e.stream_; dec_st = e.dec_stream_; ready = e.latents_ready_;
     const Spec& s = e.spec();
     const EngineOptions& o = e.options();
@@ -548,8 +548,14 @@ Batch::Batch(Engine& e, int B_, bool lm_only_) : B(B_), Bw(B_), lm_only(lm_only_
     // bf16 and int8 engines keep K and V in bf16 (half the cache traffic of the decode step); fp32 keeps f32
     kv16 = e.model().flow_wtype == W_BF16 && std::getenv("POCKET_TTS_KV_F32") == nullptr ? 1 : 0;
     const size_t kvb = kv16 ? 2 : 4;
-    lm_k.alloc(static_cast<size_t>(s.lm_layers) * B * lm_cap * D * kvb);
-    lm_v.alloc(static_cast<size_t>(s.lm_layers) * B * lm_cap * D * kvb);
+    if (pages) {
+        paged = std::make_unique<PagedCache>(s, B, kv16, *pages);
+        lm_cap = pages->max_context;
+        PTTS_HIP(hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, o.device));
+    } else {
+        lm_k.alloc(static_cast<size_t>(s.lm_layers) * B * lm_cap * D * kvb);
+        lm_v.alloc(static_cast<size_t>(s.lm_layers) * B * lm_cap * D * kvb);
+    }
     lm_pos.alloc(static_cast<size_t>(B) * 4);
     lm_pos_host.assign(B, 0);
     if (!lm_only) {
@@ -679,6 +685,10 @@ void Batch::reset(hipStream_t s) {
     PTTS_HIP(hipMemsetAsync(lm_pos.p, 0, lm_pos.bytes, s));
     PTTS_HIP(hipMemsetAsync(dec_pos.p, 0, dec_pos.bytes, s));
     std::fill(lm_pos_host.begin(), lm_pos_host.end(), 0);
+    if (paged) {
+        PTTS_HIP(hipStreamSynchronize(s));
+        paged->clear();
+    }
     std::fill(dec_pos_host.begin(), dec_pos_host.end(), 0);
     if (!lm_only)
         for (DevBuf* b : {&qbuf, &ybuf, &e0buf, &uebuf[0], &uebuf[1], &uebuf[2], &ebuf[0], &ebuf[1], &ebuf[2]})
@@ -1055,7 +1065,7 @@ void Engine::lm_rows(Batch& b, int slot0, int nb, int rpb, float* X, const int* 
     b.ensure_rows(static_cast<size_t>(nb) * rpb, s.d_model, s.lm_ffn);
     // int8 matrices exist only in the skinny kernels' layout; float and bf16 passes of up to 128 rows (one utterance's
     // voice and text) go the same way, because a tiled GEMM of that height fills 16 to 48 of the 256 CUs
-    if (model_->lm_wtype == W_I8 || (nb * rpb <= 128 && !std::getenv("POCKET_TTS_NO_SKINNY_PREFILL"))) {
+    if (model_->lm_wtype == W_I8 || b.paged || (nb * rpb <= 128 && !std::getenv("POCKET_TTS_NO_SKINNY_PREFILL"))) {
         lm_rows_skinny(b, slot0, nb, rpb, X);
         if (adv_dev) launch_advance_pos_vec(b.lm_pos.as<int>() + slot0, adv_dev, nb, b.st);
         else launch_advance_pos(b.lm_pos.as<int>() + slot0, nb, rpb, b.st);
@@ -1086,6 +1096,7 @@ void Engine::lm_rows_skinny(Batch& b, int slot0, int nb, int rpb, float* X) {
         b.pre_partial.alloc(need);
     }
     const long long layer_stride = static_cast<long long>(b.B) * b.lm_cap * D;
+    if (b.paged) b.paged->plan(slot0, nb, rpb, &b.lm_pos_host[slot0], st);
     AddNormArgs an;
     an.X = X; an.ldx = D; an.M = M; an.D = D; an.eps = s.lm_eps;
     an.g = hd_.lm[0].ln1g; an.b = hd_.lm[0].ln1b; an.H = b.h.f();
@@ -1097,6 +1108,8 @@ void Engine::lm_rows_skinny(Batch& b, int slot0, int nb, int rpb, float* X) {
         q.A = b.h.f(); q.lda = D; q.Wp = pw.qkv; q.Wp2 = pw.qkv_lo; q.wtype = wt; q.wscale = pw.s_qkv; q.M = M; q.N = 3 * D; q.K = D; q.C = b.qkv.f(); q.ldc = 3 * D;
         bind_q8_act(q, model_->q8_act, pw.ws_qkv);
         launch_skinny_gemm(q, st);
+        if (b.paged) b.paged->attend(l, b.qkv.f(), D, b.q.f(), b.att.f(), b.cus, st);
+        else {
         RopeAppendArgs r;
         const long long kv_off = static_cast<long long>(l) * layer_stride * (b.kv16 ? 2 : 4);
         r.qkv = b.qkv.f(); r.q_out = b.q.f(); r.kcache = static_cast<char*>(b.lm_k.p) + kv_off; r.vcache = static_cast<char*>(b.lm_v.p) + kv_off; r.kv16 = b.kv16;
@@ -1107,6 +1120,7 @@ void Engine::lm_rows_skinny(Batch& b, int slot0, int nb, int rpb, float* X) {
         at.q = b.q.f(); at.out = b.att.f(); at.kcache = r.kcache; at.vcache = r.vcache; at.kv16 = b.kv16; at.pos = r.pos; at.slot0 = slot0; at.rpb = rpb;
         at.M = M; at.d = D; at.heads = s.lm_heads; at.cap = b.lm_cap; at.window = 0;
         launch_attention(at, st);
+        }
         SkinnyArgs o;
         o.A = b.att.f(); o.lda = D; o.Wp = pw.out; o.Wp2 = pw.out_lo; o.wtype = wt; o.wscale = pw.s_out; o.M = M; o.N = D; o.K = D; o.splits = s_out; o.P = b.pre_partial.f();
         bind_q8_act(o, model_->q8_act, pw.ws_out);
@@ -1158,16 +1172,16 @@ void Engine::lm_step_dev(Batch& b, const float* seq_dev, float* cond_dev, float*
     int s_qkv = 1;
     if (const char* e = std::getenv("POCKET_TTS_QKV_SPLITS")) s_qkv = std::atoi(e);
     else if (B <= 64 && D % (4 * kstep) == 0) s_qkv = 4;   // measured at B = 64: 1 -> 0.568 ms per step, 2 -> 0.528, 4 -> 0.518
-    if (s_qkv < 1 || D % s_qkv || (D / s_qkv) % kstep) s_qkv = 1;
+    if (s_qkv < 1 || D % s_qkv || (D / s_qkv) % kstep || b.paged) s_qkv = 1;   // the paged attention reads finished rows
     if (b.qkv.bytes < static_cast<size_t>(s_qkv) * B * 3 * D * 4) throw std::runtime_error("QKV slab buffer too small");
     if (b.partial.bytes < static_cast<size_t>(std::max(s_out, s_ff2)) * B * D * 4) throw std::runtime_error("split-K slab buffer too small");
     // int8 engine: every matrix input of the step is quantised by the kernel that produces it (add & norm, attention,
     // the FFN-1 epilogue), so the products read int8 rows and stage nothing
     // (block scheme only: in the dynamic uint8 scheme the products quantise their rows themselves)
-    const bool preq = wt == W_I8 && model_->q8_act == 0 && b.q_rows > 0 && !std::getenv("POCKET_TTS_Q8_STAGED");
+    const bool preq = wt == W_I8 && model_->q8_act == 0 && b.q_rows > 0 && !b.paged && !std::getenv("POCKET_TTS_Q8_STAGED");
     // dynamic uint8 scheme: the producers leave the (min, max) of the rows they write, so that the products need not scan
     // their rows over the full K before quantising them (POCKET_TTS_Q8_STAGED=1: the products scan)
-    const bool dyn_mm = wt == W_I8 && model_->q8_act == 1 && b.mm_h.p && !std::getenv("POCKET_TTS_Q8_STAGED");
+    const bool dyn_mm = wt == W_I8 && model_->q8_act == 1 && b.mm_h.p && !b.paged && !std::getenv("POCKET_TTS_Q8_STAGED");
     AddNormArgs an;
     an.X = b.x.f(); an.ldx = D; an.M = B; an.D = D; an.eps = s.lm_eps;
     an.g = hd_.lm[0].ln1g; an.b = hd_.lm[0].ln1b; an.H = b.h.f();
@@ -1189,6 +1203,8 @@ void Engine::lm_step_dev(Batch& b, const float* seq_dev, float* cond_dev, float*
         bind_q8_act(q, model_->q8_act, pw.ws_qkv);
         if (dyn_mm) { q.a_mm = b.mm_h.f(); q.mm_parts = 1; }
         launch_skinny_gemm(q, b.st);
+        if (b.paged) b.paged->attend(l, b.qkv.f(), D, b.q.f(), b.att.f(), b.cus, b.st);
+        else {
         AttnDecodeArgs at;
         const long long kv_off = static_cast<long long>(l) * layer_stride * (b.kv16 ? 2 : 4);
         at.qkv = b.qkv.f(); at.qkv_splits = s_qkv; at.kcache = static_cast<char*>(b.lm_k.p) + kv_off; at.vcache = static_cast<char*>(b.lm_v.p) + kv_off; at.kv16 = b.kv16;
@@ -1198,6 +1214,7 @@ void Engine::lm_step_dev(Batch& b, const float* seq_dev, float* cond_dev, float*
         if (preq) { at.out = nullptr; at.out_q = b.attq.as<signed char>(); at.out_d = b.attd.f(); at.Mq = b.q_rows; }
         if (dyn_mm) at.out_mm = b.mm_att.f();
         launch_attn_decode(at, b.st);
+        }
         SkinnyArgs o;
         o.A = b.att.f(); o.lda = D; o.Wp = pw.out; o.Wp2 = pw.out_lo; o.wtype = wt; o.wscale = pw.s_out; o.M = B; o.N = D; o.K = D; o.splits = s_out; o.P = b.partial.f();
         if (preq) { o.A = nullptr; o.Aq = b.attq.as<signed char>(); o.ldaq = D; o.Ad = b.attd.f(); o.Mq = b.q_rows; }

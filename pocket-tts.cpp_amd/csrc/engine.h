@@ -149,6 +149,34 @@ using ChunkCallback = std::function<void(const float*, int, bool)>;
 
 class Batch;
 
+// Keys and values of an LM state in pages (engine_paged.cpp).
+struct PagedOptions { int pages = 0, page_size = 16, max_context = 0, window = 0, sinks = 0; };
+class PagedCache {
+public:
+    PagedCache(const Spec& s, int slots, int kv16, const PagedOptions& o);
+    ~PagedCache();
+    void clear();
+    void check_room(int slot, int length, int rows, int chunk) const;
+    void plan(int slot0, int nb, int rows, const int* pos, hipStream_t st);
+    void attend(int layer, const float* qkv, int d, float* q, float* out, int cus, hipStream_t st);
+    void share(int from, int to, int rows, int from_length, hipStream_t st);
+    void check_status();
+    int free_count() const { return static_cast<int>(free_pages.size()); }
+    const PagedOptions opt;
+
+private:
+    void release(int page);
+    void drop(int slot);
+    void drop_behind_window(int slot, int length);
+    int kv16, layers, heads, width = 0, most = 0, now_slot0 = 0, now_nb = 0, now_rows = 0;
+    size_t layer_bytes = 0;
+    DevBuf k, v, table, ints, freq, slot_map, positions, work;
+    int *cached = nullptr, *arriving = nullptr, *fresh = nullptr, *cu = nullptr, *kv_len = nullptr, *counts = nullptr, *status = nullptr;
+    int* host = nullptr;                       // pinned: cached, arriving and fresh pages of a call
+    std::vector<int> free_pages, uses;         // uses: slots that hold a page
+    std::vector<std::vector<int>> held;        // pages of each slot in order, -1: given back
+};
+
 // A staged batch: the utterances cut into contiguous parts, each part a lock-step Batch that runs on its own
 // stream ("lane").  The frame loop is a chain of small dependent launches that leaves most of the chip idle,
 // so several parts in flight at once multiply throughput at nearly unchanged per-frame latency.
@@ -220,6 +248,8 @@ public:
     // ---- graph-level entry points (one per reference Run call site), host buffers in and out ----
     void op_text_conditioner(const int64_t* ids, int T, float* out);
     Batch* batch_new(int B);
+    Batch* batch_new_paged(int B, const PagedOptions& o);
+    void op_state_share(Batch* b, int from, int to, int rows);
     void batch_free(Batch* b);
     void batch_reset(Batch* b);
     void op_lm_prefill(Batch* b, int slot, const float* emb, int rows);
@@ -365,7 +395,8 @@ private:
 class Batch {
 public:
     // lm_only: a staging batch for prefill passes (LM state and transformer scratch only)
-    Batch(Engine& e, int B, bool lm_only = false);
+    // paged: keys and values in a pool of pages instead of the fixed LM cache (states of the graph-level calls only)
+    Batch(Engine& e, int B, bool lm_only = false, const PagedOptions* paged = nullptr);
     void reset(hipStream_t s);
 
     int B;            // capacity: slots, and the slot stride of every state buffer
@@ -384,6 +415,8 @@ public:
     // LM state
     int kv16 = 0;           // 1: K/V caches hold bf16 (bf16 and int8 engines), 0: f32
     DevBuf lm_k, lm_v;      // [layers][B][lm_cap][d_model]
+    std::unique_ptr<PagedCache> paged;   // instead of lm_k, lm_v
+    int cus = 0;            // compute units of the device (paged)
     DevBuf lm_pos;          // int[B]
     std::vector<int> lm_pos_host;
     // decoder state

@@ -767,13 +767,15 @@ void Engine::op_lm_prefill(Batch* b, int slot, const float* emb, int rows) {
     std::lock_guard<std::mutex> guard(mu_);
     PTTS_HIP(hipSetDevice(opt_.device));
     if (slot < 0 || slot >= b->B) throw std::runtime_error("lm_prefill: slot out of range");
-    const int D = spec().d_model, chunk = 256;
+    const int D = spec().d_model, chunk = b->paged ? 128 : 256;   // paged passes run on the short-pass kernels
+    if (b->paged) b->paged->check_room(slot, b->lm_pos_host[slot], rows, chunk);
     for (int r0 = 0; r0 < rows; r0 += chunk) {
         int n = std::min(chunk, rows - r0);
         PTTS_HIP(hipMemcpyAsync(b->x.p, emb + static_cast<size_t>(r0) * D, static_cast<size_t>(n) * D * 4, hipMemcpyHostToDevice, stream_));
         lm_rows(*b, slot, 1, n, b->x.f());
     }
     PTTS_HIP(hipStreamSynchronize(stream_));
+    if (b->paged) b->paged->check_status();
 }
 
 void Engine::op_lm_step(Batch* b, const float* seq, float* cond, float* eos) {
@@ -781,11 +783,13 @@ void Engine::op_lm_step(Batch* b, const float* seq, float* cond, float* eos) {
     PTTS_HIP(hipSetDevice(opt_.device));
     const Spec& s = spec();
     PTTS_HIP(hipMemcpyAsync(b->xcur.p, seq, static_cast<size_t>(b->B) * s.latent * 4, hipMemcpyHostToDevice, stream_));
+    if (b->paged) b->paged->plan(0, b->B, 1, b->lm_pos_host.data(), b->st);
     lm_bookkeeping(*b);
     lm_step_dev(*b, b->xcur.f(), b->cond.f(), b->eos.f());
     PTTS_HIP(hipMemcpyAsync(cond, b->cond.p, static_cast<size_t>(b->B) * s.d_model * 4, hipMemcpyDeviceToHost, stream_));
     PTTS_HIP(hipMemcpyAsync(eos, b->eos.p, static_cast<size_t>(b->B) * 4, hipMemcpyDeviceToHost, stream_));
     PTTS_HIP(hipStreamSynchronize(stream_));
+    if (b->paged) b->paged->check_status();
 }
 
 void Engine::op_flow_euler(const float* cond, const float* x0, int B, float* x_out) {

@@ -50,7 +50,7 @@ EXT_SYMBOLS = [
     "pocket_tts_create_ex", "pocket_tts_dims", "pocket_tts_voice_from_embeddings", "pocket_tts_voice_frames",
     "pocket_tts_voice_data", "pocket_tts_encode_voices", "pocket_tts_generate_batch", "pocket_tts_generate_ids", "pocket_tts_generate_ids_queued", "pocket_tts_streaming_ids",
     "pocket_tts_stage_ids", "pocket_tts_run_staged", "pocket_tts_fetch_staged",
-    "pocket_tts_tokenize", "ptts_text_conditioner", "ptts_state_new", "ptts_state_free", "ptts_state_reset",
+    "pocket_tts_tokenize", "ptts_text_conditioner", "ptts_state_new", "ptts_state_new_paged", "ptts_state_share", "ptts_state_free_pages", "ptts_state_free", "ptts_state_reset",
     "ptts_lm_prefill", "ptts_lm_step", "ptts_flow_euler", "ptts_flow_euler_noalloc", "ptts_flow_euler_noalloc_capacity", "ptts_mimi_decode", "ptts_mimi_encode", "ptts_mimi_encode_batch",
     "ptts_phase_timing", "ptts_phase_times", "ptts_weight_bytes", "ptts_scheduler_stats", "ptts_scheduler_stats_ex", "ptts_engine_count", "ptts_q8_linear", "ptts_q8_linear_q", "ptts_q8_linear_dyn", "ptts_bf16_linear",
     "ptts_tokenizer_new", "ptts_tokenizer_free", "ptts_tokenizer_vocab", "ptts_tokenizer_encode",
@@ -133,6 +133,9 @@ def load() -> C.CDLL:
     L.pocket_tts_streaming_ids.argtypes = [vp, i64p, ci, f32p, ci, vp, ci, CHUNK_CB, vp]
     L.ptts_text_conditioner.restype = ci; L.ptts_text_conditioner.argtypes = [vp, i64p, ci, f32p]
     L.ptts_state_new.restype = vp; L.ptts_state_new.argtypes = [vp, ci]
+    L.ptts_state_new_paged.restype = vp; L.ptts_state_new_paged.argtypes = [vp, ci, ci, ci, ci, ci, ci]
+    L.ptts_state_share.restype = ci; L.ptts_state_share.argtypes = [vp, vp, ci, ci, ci]
+    L.ptts_state_free_pages.restype = ci; L.ptts_state_free_pages.argtypes = [vp, vp]
     L.ptts_state_free.restype = None; L.ptts_state_free.argtypes = [vp, vp]
     L.ptts_state_reset.restype = ci; L.ptts_state_reset.argtypes = [vp, vp]
     L.ptts_lm_prefill.restype = ci; L.ptts_lm_prefill.argtypes = [vp, vp, ci, f32p, ci]
@@ -252,13 +255,23 @@ def _check(rc: int, what: str) -> int:
 
 
 class State:
-    """Recurrent state of `batch` lock-step utterances."""
+    """Recurrent state of `batch` lock-step utterances; with `pages`, the LM's keys and values in a pool of pages (ptts_state_new_paged)."""
 
-    def __init__(self, eng: "Engine", batch: int):
+    def __init__(self, eng: "Engine", batch: int, pages: int = 0, page_size: int = 16, max_context: int = 0, window: int = 0, sinks: int = 0):
         self.eng, self.batch = eng, batch
-        self.p = eng.L.ptts_state_new(eng.h, batch)
+        if pages:
+            self.p = eng.L.ptts_state_new_paged(eng.h, batch, pages, page_size, max_context or pages * page_size, window, sinks)
+        else:
+            self.p = eng.L.ptts_state_new(eng.h, batch)
         if not self.p:
             raise PttsError(f"state_new: {last_error()}")
+
+    def share(self, from_slot: int, to_slot: int, rows: int):
+        """Paged states: to_slot begins anew with the first `rows` rows of from_slot."""
+        _check(self.eng.L.ptts_state_share(self.eng.h, self.p, from_slot, to_slot, rows), "state_share")
+
+    def free_pages(self) -> int:
+        return _check(self.eng.L.ptts_state_free_pages(self.eng.h, self.p), "state_free_pages")
 
     def reset(self):
         _check(self.eng.L.ptts_state_reset(self.eng.h, self.p), "state_reset")
@@ -323,6 +336,12 @@ class Engine:
 
     def state(self, batch: int) -> State:
         return State(self, batch)
+
+    def paged_state(self, batch: int, pages: int, page_size: int = 16, max_context: int = 0, window: int = 0, sinks: int = 0) -> State:
+        """LM state in a pool of pages (max_context 0: what the pool holds)."""
+        if pages <= 0:
+            raise PttsError("paged_state: pages must be positive")
+        return State(self, batch, pages, page_size, max_context, window, sinks)
 
     def lm_prefill(self, st: State, slot: int, emb) -> None:
         emb = np.ascontiguousarray(emb, np.float32)
