@@ -12,6 +12,7 @@
 #include "onnx_reader.h"
 #include "engine.h"
 #include "paged.h"
+#include "rotary_frequencies.h"
 #include "pocket_tts/audio_utils.hpp"
 #include "pocket_tts/pocket_tts.hpp"
 #include "pocket_tts/pocket_tts_amd.h"
@@ -736,7 +737,6 @@ POCKET_TTS_API int ptts_paged_plan(const PttsPagedPlan* plan, int device, void* 
 
 POCKET_TTS_API int ptts_rotary_frequencies(int rot_dim, double base, int scaling, double factor, double trained, double fast, double slow,
                                            double* out, float* magnitude) {
-    if (!out || rot_dim < 2 || rot_dim % 2) { set_error("Invalid parameters"); return -1; }
     return guarded("rotary_frequencies: ", [&] {
         ptts::rotary_frequencies(rot_dim, base, scaling, factor, trained, fast, slow, out, magnitude);
         return 0;

@@ -10,6 +10,7 @@
 
 #include "engine.h"
 #include "paged.h"
+#include "rotary_frequencies.h"
 
 namespace ptts {
 

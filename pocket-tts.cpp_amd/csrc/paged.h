@@ -17,10 +17,6 @@ void launch_rotary_append(const PttsRotaryAppend& a, hipStream_t s);
 long long paged_attention_workspace(const PttsPagedAttention& a, int cus);
 void launch_paged_attention(const PttsPagedAttention& a, int cus, hipStream_t s);
 
-// Host: frequencies in radians per position and the magnitude of the rotated values (pocket_tts_amd.h).
-void rotary_frequencies(int rot_dim, double base, int scaling, double factor, double trained, double fast, double slow, double* out,
-                        float* magnitude);
-
 // The part of the checks that two of them share.
 void check_pages(const PttsPages& p, const char* who);
 

@@ -11,9 +11,11 @@
 #include <cstdint>
 #include <cstdio>
 #include <cstring>
+#include <exception>
 #include <initializer_list>
 
 #include "pocket_tts/pocket_tts_amd.h"
+#include "rotary_frequencies.h"
 
 namespace {
 
@@ -551,6 +553,22 @@ PyType_Spec g_device_array_spec = {"ptts_paged.DeviceArray", sizeof(DeviceArray)
 
 // ------------------------------------------------------------------ module
 
+// _frequencies(rot_dim, base, scaling, factor, trained, fast, slow, address of rot_dim / 2 doubles) -> magnitude
+PyObject* frequencies(PyObject*, PyObject* args) {
+    int rot_dim, scaling;
+    double base, factor, trained, fast, slow;
+    unsigned long long out;
+    if (!PyArg_ParseTuple(args, "ididdddK", &rot_dim, &base, &scaling, &factor, &trained, &fast, &slow, &out)) return nullptr;
+    try {
+        float magnitude;
+        ptts::rotary_frequencies(rot_dim, base, scaling, factor, trained, fast, slow, reinterpret_cast<double*>(out), &magnitude);
+        return PyFloat_FromDouble(magnitude);
+    } catch (const std::exception& e) {
+        PyErr_SetString(g_error, e.what());
+        return nullptr;
+    }
+}
+
 PyObject* setup(PyObject*, PyObject* args) {
     PyObject *error, *bind, *allocate;
     if (!PyArg_ParseTuple(args, "OOO", &error, &bind, &allocate)) return nullptr;
@@ -596,6 +614,7 @@ PyMethodDef g_methods[] = {
      "workspace: any contiguous array of at least attention_workspace() bytes; None: torch's allocator provides it (torch tensors only)."},
     {"setup", setup, METH_VARARGS, nullptr},
     {"bind", bind, METH_VARARGS, nullptr},
+    {"_frequencies", frequencies, METH_VARARGS, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_ptts_paged", "C side of ptts_paged", -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 

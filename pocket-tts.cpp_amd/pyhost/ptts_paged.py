@@ -54,12 +54,10 @@ _c.setup(PttsError, _bind, _allocate)
 def frequencies(rot_dim: int, base: float = 10000.0, scaling: str = "none", factor: float = 1.0, trained: float = 0.0, fast: float = 32.0,
                 slow: float = 1.0) -> Tuple[np.ndarray, float]:
     """(float64 [rot_dim / 2] radians per position, magnitude) for rotary_append; scaling: "none", "linear" (positions divided by
-    factor), "base" (stretched base) or "parts" (ptts_rotary_frequencies).  Host only."""
+    factor), "base" (stretched base) or "parts" (ptts_rotary_frequencies).  Host only: loads no
+    library."""
     names = ("none", "linear", "base", "parts")
     if scaling not in names:
         raise PttsError(f"scaling: one of {', '.join(names)}")
     out = np.empty(max(rot_dim // 2, 1), np.float64)
-    mag = C.c_float()
-    if ptts_lib.load().ptts_rotary_frequencies(rot_dim, base, names.index(scaling), factor, trained, fast, slow, out, C.byref(mag)) < 0:
-        raise PttsError(ptts_lib.last_error())
-    return out, float(mag.value)
+    return out, _c._frequencies(rot_dim, base, names.index(scaling), factor, trained, fast, slow, out.ctypes.data)
