@@ -20,6 +20,7 @@ namespace ptts {
 typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
 typedef __attribute__((ext_vector_type(4))) __bf16 bf16x4;
 typedef __attribute__((ext_vector_type(16))) float f32x16;
+typedef __attribute__((ext_vector_type(4))) unsigned u32x4;
 
 namespace {
 
@@ -67,18 +68,18 @@ __global__ __launch_bounds__(256, OCC) void gemm_lean_kernel(GemmArgs a, int gw)
     // ---- staging assignment: A as 16 (f32) or 8 (bf16) pieces per row of a K step, W as 8 pieces per row
     constexpr int APR = ABF ? 8 : 16, APT = LBM * APR / 256;     // pieces per row, pieces per thread
     constexpr int AEL = ABF ? 8 : 4;                             // elements per piece
+    // Every lane always loads: rows behind M or N repeat the last one (their results are not stored), and pieces behind K read the
+    // row's start and are zeroed when they are staged.  Loads under branches, merged with zeros behind them, had the compiler wait
+    // for each load before the next one (two-term kernel at the prefill's shapes: 131 us against 74).
     const char* aptr[APT];
     int ak[APT];
 #pragma unroll
     for (int i = 0; i < APT; ++i) {
         const int id = tid + 256 * i, row = id / APR, p = id % APR;
-        const int m = m0 + row;
+        const int m = min(m0 + row, M - 1);
         ak[i] = p * AEL;
-        aptr[i] = nullptr;
-        if (m < M) {
-            const long long off = (long long)(m / a.rpb) * a.a_bs + (long long)(m % a.rpb) * a.lda + p * AEL;
-            aptr[i] = (const char*)a.A + off * (ABF ? 2 : 4);
-        }
+        const long long off = (long long)(m / a.rpb) * a.a_bs + (long long)(m % a.rpb) * a.lda + p * AEL;
+        aptr[i] = (const char*)a.A + off * (ABF ? 2 : 4);
     }
     constexpr int WPT = LBN * 8 / 256;
     const __bf16* wptr[WPT];
@@ -87,24 +88,31 @@ __global__ __launch_bounds__(256, OCC) void gemm_lean_kernel(GemmArgs a, int gw)
     for (int i = 0; i < WPT; ++i) {
         const int id = tid + 256 * i, row = id >> 3, p = id & 7;
         wk[i] = p * 8;
-        wptr[i] = (n0 + row < N) ? (const __bf16*)a.W + (long long)(n0 + row) * K + p * 8 : nullptr;
+        wptr[i] = (const __bf16*)a.W + (long long)min(n0 + row, N - 1) * K + p * 8;
     }
-    uint4 areg[APT], wreg[WPT], wreg2[WSPLIT ? WPT : 1];
+    u32x4 areg[APT], wreg[WPT], wreg2[WSPLIT ? WPT : 1];
     const long long w2_off = WSPLIT ? (const char*)a.W2 - (const char*)a.W : 0;
     auto load_tiles = [&](int k0) {
 #pragma unroll
-        for (int i = 0; i < APT; ++i)
-            areg[i] = (aptr[i] && k0 + ak[i] < K) ? *(const uint4*)(aptr[i] + (long long)k0 * (ABF ? 2 : 4)) : make_uint4(0u, 0u, 0u, 0u);
+        for (int i = 0; i < APT; ++i) areg[i] = *(const u32x4*)(aptr[i] + (long long)(k0 + ak[i] < K ? k0 : -ak[i]) * (ABF ? 2 : 4));
 #pragma unroll
-        for (int i = 0; i < WPT; ++i)
-            wreg[i] = (wptr[i] && k0 + wk[i] < K) ? *(const uint4*)(wptr[i] + k0) : make_uint4(0u, 0u, 0u, 0u);
+        for (int i = 0; i < WPT; ++i) wreg[i] = *(const u32x4*)(wptr[i] + (k0 + wk[i] < K ? k0 : -wk[i]));
         if constexpr (WSPLIT) {
 #pragma unroll
-            for (int i = 0; i < WPT; ++i)
-                wreg2[i] = (wptr[i] && k0 + wk[i] < K) ? *(const uint4*)((const char*)(wptr[i] + k0) + w2_off) : make_uint4(0u, 0u, 0u, 0u);
+            for (int i = 0; i < WPT; ++i) wreg2[i] = *(const u32x4*)((const char*)(wptr[i] + (k0 + wk[i] < K ? k0 : -wk[i])) + w2_off);
         }
     };
-    auto store_tiles = [&]() {
+    auto store_tiles = [&](int k0) {
+        if (k0 + LBK > K) {
+            const u32x4 zero = {0u, 0u, 0u, 0u};
+#pragma unroll
+            for (int i = 0; i < APT; ++i) areg[i] = k0 + ak[i] < K ? areg[i] : zero;
+#pragma unroll
+            for (int i = 0; i < WPT; ++i) {
+                wreg[i] = k0 + wk[i] < K ? wreg[i] : zero;
+                if constexpr (WSPLIT) wreg2[i] = k0 + wk[i] < K ? wreg2[i] : zero;
+            }
+        }
 #pragma unroll
         for (int i = 0; i < APT; ++i) {
             const int id = tid + 256 * i, row = id / APR, p = id % APR;
@@ -115,7 +123,7 @@ __global__ __launch_bounds__(256, OCC) void gemm_lean_kernel(GemmArgs a, int gw)
                     for (int e = 0; e < 8; ++e) v[e] = (__bf16)act_apply((float)v[e], a.a_act);
                     *(bf16x8*)&As[row * LLD + p * 8] = v;
                 } else {
-                    *(uint4*)&As[row * LLD + p * 8] = areg[i];
+                    *(u32x4*)&As[row * LLD + p * 8] = areg[i];
                 }
             } else {
                 float4 v = __builtin_bit_cast(float4, areg[i]);
@@ -136,8 +144,8 @@ __global__ __launch_bounds__(256, OCC) void gemm_lean_kernel(GemmArgs a, int gw)
 #pragma unroll
         for (int i = 0; i < WPT; ++i) {
             const int id = tid + 256 * i, row = id >> 3, p = id & 7;
-            *(uint4*)&Ws[row * LLD + p * 8] = wreg[i];
-            if constexpr (WSPLIT) *(uint4*)&Wl[row * LLD + p * 8] = wreg2[i];
+            *(u32x4*)&Ws[row * LLD + p * 8] = wreg[i];
+            if constexpr (WSPLIT) *(u32x4*)&Wl[row * LLD + p * 8] = wreg2[i];
         }
     };
 
@@ -152,7 +160,7 @@ __global__ __launch_bounds__(256, OCC) void gemm_lean_kernel(GemmArgs a, int gw)
     const int lr = lane & 31, lh = lane >> 5;
     load_tiles(0);
     for (int k0 = 0; k0 < K; k0 += LBK) {
-        store_tiles();
+        store_tiles(k0);
         __syncthreads();
         if (k0 + LBK < K) load_tiles(k0 + LBK);
 #pragma unroll
@@ -270,7 +278,7 @@ void launch_gemm_lean(const GemmArgs& a, hipStream_t s) {
         if (a.c_bf16) hipLaunchKernelGGL((gemm_lean_kernel<true, true, false>), grid, block, 0, s, a, gw);
         else hipLaunchKernelGGL((gemm_lean_kernel<true, false, false>), grid, block, 0, s, a, gw);
     } else {
-        // f32 rows in, K of at most 1024: three workgroups per CU (168 registers, 28 bytes of scratch per lane) hide more of
+        // f32 rows in, K of at most 1024: three workgroups per CU (168 registers, 32 bytes of scratch per lane) hide more of
         // the load latency than two; with longer K loops the spilled words cost more than that buys (measured per shape).
         static const int occ3 = [] { const char* e = std::getenv("POCKET_TTS_GEMM_OCC3"); return e ? std::atoi(e) : 1; }();
         if (occ3 && a.K <= 1024) {
