@@ -15,8 +15,9 @@
 // them in.  Softmax statistics and both sums are float32; the weights are rounded once, to the rows' type, because the matrix
 // instructions take both operands in one type (at most half a step of the type on each weight; float rows keep float weights).
 //
-// The running maximum is a reference that lags: sums are rescaled only when a score passes it by 2^8, which leaves every weight
-// below 2^8, far inside float16, and saves most rescales.
+// The running maximum is a reference that lags: sums are rescaled only when a score passes it by 2^8, which saves most rescales.
+// Float16 weights are kept 2^7 times larger (at most 2^15, inside the type), so that a weight has to lie 2^-21 below the largest
+// before it loses bits and 2^-32 below before it is lost; bf16 has float32's range and needs none of this.
 #include <algorithm>
 #include <cmath>
 #include <stdexcept>
@@ -32,6 +33,7 @@ namespace {
 constexpr int kChunkRows = 128, kChunkKeys = 64;   // chunk kernel: packed rows of a workgroup, keys of a block
 constexpr int kFewRows = 16;                       // few kernel: packed rows of a workgroup
 constexpr float kLn2 = 0.69314718055994531f, kLag = 8.0f;
+template <typename T> constexpr float kLift = std::is_same<T, _Float16>::value ? 7.0f : 0.0f;
 
 // How a call is cut: which forms run, over how many tiles, into how many splits of the keys.
 struct Cut {
@@ -220,7 +222,7 @@ template <typename T, int N> __device__ __forceinline__ void clean(unsigned (&w)
 }
 __device__ __forceinline__ float add_not_finite(float sum, float v) { return fabsf(v) < INFINITY ? sum : sum + v; }
 
-// exp2 of what is at most kLag; denormals flush to zero
+// exp2 of what is at most kLag + kLift; denormals flush to zero
 __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // ------------------------------------------------------------------ chunk
@@ -392,8 +394,8 @@ template <typename T, int DH> __device__ __forceinline__ void chunk_body(const A
 #pragma unroll
             for (int r = 0; r < 16; ++r) best = fmaxf(best, s[b][r]);
         best = max_half(best) * a.scale2;
-        if (__any(best > top + kLag)) {
-            const float next = fmaxf(top, best), fade = top == -INFINITY ? 0.f : exp2_of(top - next);
+        if (__any(best > top + (kLag + kLift<T>))) {
+            const float next = fmaxf(top, best - kLift<T>), fade = top == -INFINITY ? 0.f : exp2_of(top - next);
             top = next;
             sum *= fade;
 #pragma unroll
@@ -631,8 +633,8 @@ template <typename T, typename C, int DH, bool kFull> __device__ __forceinline__
 #pragma unroll
             for (int r = 0; r < 4; ++r) best = fmaxf(best, s[b][r]);
         best = max_rows(best) * a.scale2;
-        if (__any(best > top + kLag)) {
-            const float next = fmaxf(top, best), fade = top == -INFINITY ? 0.f : exp2_of(top - next);
+        if (__any(best > top + (kLag + kLift<T>))) {
+            const float next = fmaxf(top, best - kLift<T>), fade = top == -INFINITY ? 0.f : exp2_of(top - next);
             top = next;
             sum *= fade;
 #pragma unroll
@@ -744,7 +746,7 @@ template <typename T, typename C, int DH, bool kFull> __device__ __forceinline__
 #pragma unroll
         for (int w = 0; w < 4; ++w) big = fmaxf(big, tops[w][q]);
 #pragma unroll
-        for (int w = 0; w < 4; ++w) total += tops[w][q] == -INFINITY ? 0.f : sums[w][q] * exp2_of(tops[w][q] - big);
+        for (int w = 0; w < 4; ++w) total += tops[w][q] == -INFINITY ? sums[w][q] : sums[w][q] * exp2_of(tops[w][q] - big);     // 0 or NaN
         f32x4 v = *(f32x4*)&lds.of[0].joined[q][d];
 #pragma unroll
         for (int w = 1; w < 4; ++w) v += *(f32x4*)&lds.of[w].joined[q][d];
@@ -804,15 +806,14 @@ __device__ __forceinline__ void merge_one(const PttsPagedAttention& p, const flo
             x[j] = *(const f32x4*)(part + from * p.pages.head_dim + d);
         }
         const float next = fmaxf(fmaxf(top, fmaxf(l[0], l[1])), fmaxf(l[2], l[3]));
-        if (next == -INFINITY) continue;
-        const float fade = exp2_of(top - next);
+        const float fade = top == -INFINITY ? 1.0f : exp2_of(top - next), base = next == -INFINITY ? 0.f : next;
         top = next;
         total *= fade;
         v *= fade;
 #pragma unroll
         for (int j = 0; j < 4; ++j)
             if (l[j] != -INFINITY) {
-                const float w = exp2_of(l[j] - top);
+                const float w = exp2_of(l[j] - base);        // NaN if the split's is
                 total += w;
                 v += x[j] * w;
             }
@@ -940,6 +941,8 @@ void check_paged_attention(const PttsPagedAttention& p) {
     if (p.rows < 0 || p.rows >= 1 << 30) throw std::runtime_error(w + "rows must be 0 to 2^30 - 1");
     if (p.requests < 0 || p.requests > 65536) throw std::runtime_error(w + "requests must be 0 to 65536");
     check_pages(p.pages, "paged_attention");
+    if (p.q_heads > 0 && static_cast<long long>(p.rows) * (p.q_heads / p.pages.kv_heads) >= 1ll << 30)
+        throw std::runtime_error(w + "rows * q_heads / kv_heads must be below 2^30");
     if (p.q_type != PTTS_TYPE_F32 && p.q_type != PTTS_TYPE_BF16 && p.q_type != PTTS_TYPE_F16) throw std::runtime_error(w + "unknown type");
     if (p.pages.type != p.q_type && !(p.q_type == PTTS_TYPE_F32 && p.pages.type == PTTS_TYPE_BF16))
         throw std::runtime_error(w + "pages must have the rows' type, or bf16 under f32 rows");

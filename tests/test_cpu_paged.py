@@ -107,6 +107,12 @@ def test_attention_refusals(over, text):
             _attention(ptts_paged.attention_workspace, **over)
 
 
+def test_attention_refuses_what_passes_31_bits():
+    many = dict(q=arr((1 << 20, 2048, 64), "bfloat16"), out=arr((1 << 20, 2048, 64), "bfloat16", ptr=2 * PTR))
+    with pytest.raises(ptts_lib.PttsError, match="below 2\\^30"):
+        _attention(**many)
+
+
 def test_null_arguments():
     L = ptts_lib.load()
     assert L.ptts_paged_plan(None, 0, None) == -1

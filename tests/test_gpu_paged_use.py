@@ -352,3 +352,58 @@ def test_torch_tensors(tmp_path):
     r = subprocess.run([sys.executable, "-u", str(script)], capture_output=True, text=True, timeout=100)
     assert r.returncode == 0 and "TORCH OK" in r.stdout, r.stdout[-2000:] + r.stderr[-3000:]
     assert r.stdout.count("refused:") == 6
+
+
+def _one_request(kind, q, k, v, new, splits_wanted=True):
+    """Attention of the last `new` rows of one sequence, pages in order; returns out, lse."""
+    import ptts_paged
+    from ptts_paged import DeviceArray
+    n, kvh, dim = k.shape
+    page = 16
+    pages = -(-n // page)
+    pad = [(0, pages * page - n), (0, 0), (0, 0)]
+    d = [ref.floats(q, kind)] + [ref.floats(np.pad(x, pad).reshape(pages, page, kvh, dim), kind) for x in (k, v)]
+    out, lse = ref.floats(np.zeros(q.shape), kind), ref.Dev(np.zeros(q.shape[:2]), "float32")
+    ints = [ref.Dev(x, "int32") for x in (np.arange(pages)[None], [0, new], [n], [0])]
+    a = [x.a for x in d] + [x.a for x in ints[:3]]
+    need = ptts_paged.attention_workspace(*a, out=out.a, max_rows=new)
+    ws = ref.Dev(np.full(max(need, 16), 255), "uint8")
+    ptts_paged.attention(*a, out=out.a, lse=lse.a, max_rows=new, workspace=DeviceArray(ws.ptr, (max(need, 16) // 4,), "int32"), status=ints[3].a)
+    assert ints[3].host()[0] == 0 and (need > 0) == splits_wanted
+    return ref.from_bits(out.host(), kind), lse.host()
+
+
+@pytest.mark.parametrize("kind", ["bfloat16", "float16", "float32"])
+@pytest.mark.parametrize("n,new,splits", [(300, 1, False), (9000, 1, True), (300, 40, False), (9000, 40, True)])
+def test_queries_that_are_nan(kind, n, new, splits):
+    """A query of NaN gives NaN, in the row that holds it alone; so does a NaN that all keys of one wave hold."""
+    rng = np.random.default_rng(n + new)
+    q, k, v = (ref.rounded(rng.standard_normal((m, h, 64)), kind) for m, h in ((new, 2), (n, 1), (n, 1)))
+    splits = splits or (kind == "float32" and n > 4000)
+    q[0, 0, 5] = np.nan
+    out, lse = _one_request(kind, q, k, v, new, splits)
+    assert np.isnan(out[0, 0]).all() and np.isnan(lse[0, 0])
+    rest = np.ones((new, 2), bool)
+    rest[0, 0] = False
+    assert np.isfinite(out[rest]).all() and np.isfinite(lse[rest]).all()
+    k[32:64] = np.nan                                       # every score of one wave's step
+    out, lse = _one_request(kind, q, k, v, new, splits)
+    assert np.isnan(out).all() and np.isnan(lse).all()
+
+
+@pytest.mark.parametrize("kind", ["bfloat16", "float16", "float32"])
+@pytest.mark.parametrize("new", [1, 20])
+def test_many_small_weights_add_up(kind, new):
+    """One key far above 8000 others, each 2^-27 of it: together they are all of the result.  A weight is rounded by half a step of its type (float16: of
+    2^-24 under a factor of 2^7, so 2^-32 of the largest), the result once, and two sums of 8000 terms in float32 add 2^-10."""
+    n, dim = 8000, 64
+    q, k, v = np.zeros((new, 1, dim)), np.zeros((n, 1, dim)), np.full((n, 1, dim), 64.0)
+    q[:, 0, 0], k[7, 0, 0], v[7] = 1.0, 8.0 * 27 * np.log(2), 0.0
+    k = ref.rounded(k, kind)
+    out, lse = _one_request(kind, q, k, v, new)
+    for r in range(new):
+        seen = n - new + r + 1
+        w = np.exp(-k[7, 0, 0] / 8.0)
+        want = 64 * (seen - 1) * w / (1 + (seen - 1) * w)
+        slack = (ref.EPS[kind] + (2.0 ** -32 / w if kind == "float16" else 0.0) + ref.EPS[kind] + 2.0 ** -9) * want
+        assert (np.abs(out[r] - want) <= slack).all(), (r, out[r, 0, 0], want)
