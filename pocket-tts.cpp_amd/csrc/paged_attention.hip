@@ -8,8 +8,6 @@
 //           the one read of the keys and values)
 //   merge   joins the results of rows whose keys were cut into splits
 //
-// Batches that may hold both kinds of requests run both forms in one launch, the memory-bound one beside the other.
-//
 // All products are formed transposed, S^T = K Q^T and O^T = V^T P^T, so that a lane keeps one query for the whole kernel (its
 // running maximum and sum are scalars of the lane) and the weights leave the first product in the layout the second one takes
 // them in.  Softmax statistics and both sums are float32; the weights are rounded once, to the rows' type, because the matrix
@@ -35,28 +33,23 @@ constexpr int kFewRows = 16;                       // few kernel: packed rows of
 constexpr float kLn2 = 0.69314718055994531f, kLag = 8.0f;
 template <typename T> constexpr float kLift = std::is_same<T, _Float16>::value ? 7.0f : 0.0f;
 
-// How a call is cut: which forms run, over how many tiles, into how many splits of the keys.
+// How a call is cut: which form runs, over how many tiles, into how many splits of the keys.
 struct Cut {
-    bool chunk = false, few = false;
-    int small = 0;              // both run: requests of at most this many packed rows (one tile) go to the few form
-    long long chunk_tiles = 0, few_tiles = 0;
-    int chunk_splits = 1, few_splits = 1;
-    int chunk_least = 1, few_least = 1;               // fewest key blocks of a split
-    long long chunk_parts = 0, few_parts = 0;         // rows of one split's results in the workspace
-    long long bytes = 0;
+    bool chunk;
+    long long tiles;
+    int splits, least;          // least: fewest key blocks (chunk) or steps (few) of a split
+    long long parts, bytes;     // rows of one split's results in the workspace; its size
 };
 
 struct AttnArgs {
     PttsPagedAttention p;
     FastDiv page, group;
     float scale2;               // scale * log2(e)
-    int small;
-    unsigned few_blocks;        // workgroups of the few form; those of the chunk form follow
-    long long chunk_tiles;
-    int chunk_splits, few_splits, chunk_least, few_least;
-    // results of splits: [split][row][dim] values, normalised by the split's own sum, and [split][row] of log2 sum exp2
-    float *chunk_part, *chunk_lse, *few_part, *few_lse;
-    long long chunk_parts, few_parts;
+    long long tiles;
+    int splits, least;
+    // results of splits: [split][row][head][dim] values, normalised by the split's own sum, and [split][row][head] of log2 sum exp2
+    float *part, *lse;
+    long long parts;
 };
 
 typedef __attribute__((ext_vector_type(4))) float f32x4;
@@ -99,48 +92,39 @@ struct Tile {
 
 // Tile numbers of request i begin at cu_rows[i] * G / BM + i: its ceil(n G / BM) tiles end before those of the next request
 // begin, so a tile finds its request without prefix sums, 64 requests at a time, and a few numbers stay unused.
-// `direct`: tile i is request i's first.
-__device__ __forceinline__ bool find_tile(const AttnArgs& a, long long tile, int rows_per_tile, bool direct, Tile& t) {
+__device__ __forceinline__ bool find_tile(const AttnArgs& a, long long tile, int rows_per_tile, Tile& t) {
     const PttsPagedAttention& p = a.p;
     const int lane = threadIdx.x & 63, G = a.group.d;
     int sub, end;
-    if (direct) {
-        t.i = (int)tile;
-        sub = 0;
-        t.row0 = p.cu_rows[t.i];
-        end = p.cu_rows[t.i + 1];
-        t.len = p.kv_len[t.i];
-    } else {
-        auto first_of = [&](int i, int cu) { return (long long)cu * G / rows_per_tile + i; };
-        int lo = 0, span = p.requests;
-        while (span > 64) {
-            const int step = (span + 63) >> 6, i = lo + lane * step;
-            const bool hit = lane * step < span && first_of(i, p.cu_rows[i]) <= tile;
-            const int hits = __popcll(__ballot(hit));
-            if (hits == 0) return false;
-            const int left = span - (hits - 1) * step;
-            lo += (hits - 1) * step;
-            span = left < step ? left : step;
-        }
-        // the last round reads all that the tile needs of its request at once
-        int cu = 0, next = 0, len = 0;
-        bool hit = false;
-        if (lane < span) {
-            cu = p.cu_rows[lo + lane];
-            next = p.cu_rows[lo + lane + 1];
-            len = p.kv_len[lo + lane];
-            hit = first_of(lo + lane, cu) <= tile;
-        }
+    auto first_of = [&](int i, int cu) { return (long long)cu * G / rows_per_tile + i; };
+    int lo = 0, span = p.requests;
+    while (span > 64) {
+        const int step = (span + 63) >> 6, i = lo + lane * step;
+        const bool hit = lane * step < span && first_of(i, p.cu_rows[i]) <= tile;
         const int hits = __popcll(__ballot(hit));
         if (hits == 0) return false;
-        t.i = lo + hits - 1;
-        t.row0 = __builtin_amdgcn_readlane(cu, hits - 1);
-        end = __builtin_amdgcn_readlane(next, hits - 1);
-        t.len = __builtin_amdgcn_readlane(len, hits - 1);
-        const long long first = first_of(t.i, t.row0);
-        if (tile < first || tile - first > 0x7fffffff) return false;
-        sub = (int)(tile - first);
+        const int left = span - (hits - 1) * step;
+        lo += (hits - 1) * step;
+        span = left < step ? left : step;
     }
+    // the last round reads all that the tile needs of its request at once
+    int cu = 0, next = 0, len = 0;
+    bool hit = false;
+    if (lane < span) {
+        cu = p.cu_rows[lo + lane];
+        next = p.cu_rows[lo + lane + 1];
+        len = p.kv_len[lo + lane];
+        hit = first_of(lo + lane, cu) <= tile;
+    }
+    const int hits = __popcll(__ballot(hit));
+    if (hits == 0) return false;
+    t.i = lo + hits - 1;
+    t.row0 = __builtin_amdgcn_readlane(cu, hits - 1);
+    end = __builtin_amdgcn_readlane(next, hits - 1);
+    t.len = __builtin_amdgcn_readlane(len, hits - 1);
+    const long long first = first_of(t.i, t.row0);
+    if (tile < first || tile - first > 0x7fffffff) return false;
+    sub = (int)(tile - first);
     t.bad = 0;
     t.n = end - t.row0;
     if (t.row0 < 0 || end > p.rows || end < t.row0) {
@@ -242,7 +226,10 @@ __device__ __forceinline__ void copy16(const void* from, void* to) {
     __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) unsigned*)from, (__attribute__((address_space(3))) unsigned*)to, 16, 0, 0);
 }
 
-template <typename T, int DH> __device__ __forceinline__ void chunk_body(const AttnArgs& a, unsigned block, ChunkLds<T, DH>& lds) {
+// Three workgroups per CU where the head fits (170 registers), else two or one.
+template <typename T, int DH> __global__ __launch_bounds__(256, DH == 256 ? 1 : DH == 128 ? 2 : 3) void attention_chunk_kernel(AttnArgs a) {
+    __shared__ __attribute__((aligned(16))) ChunkLds<T, DH> lds;
+    const unsigned block = blockIdx.x;
     constexpr int kUnits = DH / 8, kPassRows = 256 / kUnits, kPasses = kChunkKeys / kPassRows, KS = DH / 16, NT = DH / 32;
     const PttsPagedAttention& p = a.p;
     const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, h = lane >> 5;
@@ -251,13 +238,12 @@ template <typename T, int DH> __device__ __forceinline__ void chunk_body(const A
     // most keys first
     const int kvh = block % p.pages.kv_heads;
     const unsigned rest = block / p.pages.kv_heads;
-    const int splits = a.chunk_splits, split = rest % splits;
+    const int splits = a.splits, split = rest % splits;
     Tile t;
-    if (!find_tile(a, a.chunk_tiles - 1 - rest / splits, kChunkRows, 0, t)) return;
+    if (!find_tile(a, a.tiles - 1 - rest / splits, kChunkRows, t)) return;
     const int G = a.group.d, dim = p.pages.head_dim;
-    if ((long long)t.n * G <= a.small) return;
     const Blocks list(t, p.sinks, kChunkKeys);
-    const int per = max(a.chunk_least, (list.count + splits - 1) / splits);
+    const int per = max(a.least, (list.count + splits - 1) / splits);
     const int u0 = split * per, u1 = min(list.count, u0 + per);
 
     // this lane's query, and the positions of this wave's rows
@@ -463,8 +449,8 @@ template <typename T, int DH> __device__ __forceinline__ void chunk_body(const A
                 }
         if (p.lse && h == 0) p.lse[(long long)row * p.lse_row_stride + head] = lse2 * kLn2;
     } else {
-        const long long at = split * a.chunk_parts + (long long)row * p.q_heads + head;
-        float* part = a.chunk_part + at * dim + 4 * h;
+        const long long at = split * a.parts + (long long)row * p.q_heads + head;
+        float* part = a.part + at * dim + 4 * h;
         if (sum != 0.f)
 #pragma unroll
             for (int n = 0; n < NT; ++n)
@@ -472,7 +458,7 @@ template <typename T, int DH> __device__ __forceinline__ void chunk_body(const A
                 for (int q = 0; q < 4; ++q)
                     if (32 * n + 8 * q < dim)
                         *(f32x4*)(part + 32 * n + 8 * q) = f32x4{o[n][4 * q] * inv, o[n][4 * q + 1] * inv, o[n][4 * q + 2] * inv, o[n][4 * q + 3] * inv};
-        if (h == 0) a.chunk_lse[at] = lse2;
+        if (h == 0) a.lse[at] = lse2;
     }
 }
 
@@ -500,7 +486,10 @@ template <int DH> struct FewLds {
 };
 
 // kFull: the head fills DH, so that no lane's values lie behind it.
-template <typename T, typename C, int DH, bool kFull> __device__ __forceinline__ void few_body(const AttnArgs& a, unsigned block, FewLds<DH>& lds) {
+template <typename T, typename C, int DH, bool kFull>
+__global__ __launch_bounds__(256, DH == 256 ? 1 : DH == 128 ? 2 : 3) void attention_few_kernel(AttnArgs a) {
+    __shared__ __attribute__((aligned(16))) FewLds<DH> lds;
+    const unsigned block = blockIdx.x;
     using S = Step<T, C, DH>;
     constexpr int NA = S::NA, CPL = S::CPL, KS = S::KS, KW = S::KW, VW = S::VW, VN = S::VN, kWaveKeys = 16 * NA, kKeys = 4 * kWaveKeys;
     constexpr bool kFloat = S::kFloat;
@@ -510,13 +499,12 @@ template <typename T, typename C, int DH, bool kFull> __device__ __forceinline__
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);   // matrix instructions ignore the lane mask: every branch around one is scalar
     const int kvh = block % p.pages.kv_heads;
     const unsigned rest = block / p.pages.kv_heads;
-    const int splits = a.few_splits, split = rest % splits;
+    const int splits = a.splits, split = rest % splits;
     Tile t;
-    if (!find_tile(a, rest / splits, kFewRows, a.small > 0, t)) return;
+    if (!find_tile(a, rest / splits, kFewRows, t)) return;
     const int G = a.group.d, dim = p.pages.head_dim;
-    if (a.small > 0 && (long long)t.n * G > a.small) return;
     const Blocks list(t, p.sinks, kKeys);
-    const int per = max(a.few_least, (list.count + splits - 1) / splits);
+    const int per = max(a.least, (list.count + splits - 1) / splits);
     const int u0 = split * per, u1 = min(list.count, u0 + per);
 
     const int m = min(t.m0 + li, t.m1 - 1), tok = a.group.div(m), head = kvh * G + m - tok * G, row = t.row0 + tok, pos = t.pos0 + tok;
@@ -760,64 +748,54 @@ template <typename T, typename C, int DH, bool kFull> __device__ __forceinline__
             *(x4<T>*)((T*)p.out + rq * p.out_row_stride + (long long)hq * p.out_head_stride + d) = w;
             if (p.lse && d == 0) p.lse[rq * p.lse_row_stride + hq] = lse2 * kLn2;
         } else {
-            const long long at = split * a.few_parts + (a.small > 0 ? ((long long)t.i * p.pages.kv_heads + kvh) * kFewRows + mq : rq * p.q_heads + hq);
-            if (total != 0.f) *(f32x4*)(a.few_part + at * dim + d) = v * inv;
-            if (d == 0) a.few_lse[at] = lse2;
+            const long long at = split * a.parts + rq * p.q_heads + hq;
+            if (total != 0.f) *(f32x4*)(a.part + at * dim + d) = v * inv;
+            if (d == 0) a.lse[at] = lse2;
         }
     }
-}
-
-// The forms' entries.  A launch of the few form alone does not carry the chunk form's registers and LDS.
-template <typename T, typename C, int DH, bool kFull> __global__ __launch_bounds__(256, DH == 256 ? 1 : DH == 128 ? 2 : 3) void attention_few_kernel(AttnArgs a) {
-    __shared__ __attribute__((aligned(16))) FewLds<DH> lds;
-    few_body<T, C, DH, kFull>(a, blockIdx.x, lds);
-}
-// Three workgroups per CU where the head fits (170 registers), else two.
-template <typename T, int DH> __global__ __launch_bounds__(256, DH == 256 ? 1 : DH == 128 ? 2 : 3) void attention_chunk_kernel(AttnArgs a) {
-    __shared__ __attribute__((aligned(16))) ChunkLds<T, DH> lds;
-    chunk_body<T, DH>(a, blockIdx.x, lds);
-}
-template <typename T, int DH, bool kFull> __global__ __launch_bounds__(256, DH == 256 ? 1 : DH == 128 ? 2 : 3) void attention_both_kernel(AttnArgs a) {
-    __shared__ __attribute__((aligned(16))) union Lds {
-        ChunkLds<T, DH> chunk;
-        FewLds<DH> few;
-        __device__ Lds() {}
-    } lds;
-    if (blockIdx.x < a.few_blocks) few_body<T, T, DH, kFull>(a, blockIdx.x, lds.few);
-    else chunk_body<T, DH>(a, blockIdx.x - a.few_blocks, lds.chunk);
 }
 
 // ------------------------------------------------------------------ merge
 
+// `Many` splits taken in: top, total and v are the state so far.  Their reads are on their way together; a split that saw nothing wrote no
+// values.
+template <int Many>
+__device__ __forceinline__ void merge_some(const float* part, const float* lse, long long stride, int s, int splits, long long at, int dim, int d, float& top,
+                                           float& total, f32x4& v) {
+    float l[Many], next = top;
+    f32x4 x[Many];
+#pragma unroll
+    for (int j = 0; j < Many; ++j) {
+        const long long from = min(s + j, splits - 1) * stride + at;
+        l[j] = s + j < splits ? lse[from] : -INFINITY;
+        x[j] = *(const f32x4*)(part + from * dim + d);
+    }
+#pragma unroll
+    for (int j = 0; j < Many; ++j) next = fmaxf(next, l[j]);
+    const float fade = top == -INFINITY ? 1.0f : exp2_of(top - next), base = next == -INFINITY ? 0.f : next;
+    top = next;
+    total *= fade;
+    v *= fade;
+#pragma unroll
+    for (int j = 0; j < Many; ++j)
+        if (l[j] != -INFINITY) {
+            const float w = exp2_of(l[j] - base);        // NaN if the split's is
+            total += w;
+            v += x[j] * w;
+        }
+}
+
 // out = sum over splits of exp2(lse_s - lse) part_s, four values a thread.
 template <typename T>
-__device__ __forceinline__ void merge_one(const PttsPagedAttention& p, const float* part, const float* lse, long long stride, int splits, long long at, long long row,
-                                          int head, int d) {
-    // four splits at a time, so that their reads are on their way together; a split that saw nothing wrote no values
+__device__ __forceinline__ void merge_one(const AttnArgs& a, long long row, int head, int d) {
+    const PttsPagedAttention& p = a.p;
+    const int splits = a.splits;
+    const long long at = row * p.q_heads + head;
     float top = -INFINITY, total = 0.f;
     f32x4 v = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < splits; s += 4) {
-        float l[4];
-        f32x4 x[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const long long from = min(s + j, splits - 1) * stride + at;
-            l[j] = s + j < splits ? lse[from] : -INFINITY;
-            x[j] = *(const f32x4*)(part + from * p.pages.head_dim + d);
-        }
-        const float next = fmaxf(fmaxf(top, fmaxf(l[0], l[1])), fmaxf(l[2], l[3]));
-        const float fade = top == -INFINITY ? 1.0f : exp2_of(top - next), base = next == -INFINITY ? 0.f : next;
-        top = next;
-        total *= fade;
-        v *= fade;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (l[j] != -INFINITY) {
-                const float w = exp2_of(l[j] - base);        // NaN if the split's is
-                total += w;
-                v += x[j] * w;
-            }
-    }
+    int s = 0;
+    for (; s + 4 < splits; s += 16) merge_some<16>(a.part, a.lse, a.parts, s, splits, at, p.pages.head_dim, d, top, total, v);
+    if (s < splits) merge_some<4>(a.part, a.lse, a.parts, s, splits, at, p.pages.head_dim, d, top, total, v);
     const float inv = total == 0.f ? 0.f : 1.0f / total;
     x4<T> y;
 #pragma unroll
@@ -826,25 +804,11 @@ __device__ __forceinline__ void merge_one(const PttsPagedAttention& p, const flo
     if (p.lse && d == 0) p.lse[row * p.lse_row_stride + head] = total == 0.f ? -INFINITY : (top + __log2f(total)) * kLn2;
 }
 
-// Workgroups (x) 0 .. request_blocks - 1: the few form's one tile of a request (both forms ran); the others: one row each.  Workgroups
-// along y share a row's heads.
-template <typename T>
-__global__ __launch_bounds__(256) void attention_merge_kernel(AttnArgs a, unsigned request_blocks, int row_splits, const float* row_part, const float* row_lse, long long row_parts) {
+// A row for each workgroup in x; workgroups along y share its heads.
+template <typename T> __global__ __launch_bounds__(256) void attention_merge_kernel(AttnArgs a) {
     const PttsPagedAttention& p = a.p;
-    const int G = a.group.d, quads = p.pages.head_dim / 4;
-    if (blockIdx.x < request_blocks) {
-        const int i = blockIdx.x, r0 = p.cu_rows[i], r1 = p.cu_rows[i + 1];
-        if (r0 < 0 || r1 > p.rows || r1 <= r0 || (long long)(r1 - r0) * G > a.small) return;
-        const int packed = (r1 - r0) * G, n = packed * p.pages.kv_heads * quads;
-        const int x = blockIdx.y * 256 + threadIdx.x;
-        if (x < n) {
-            const int q = x / quads, kvh = q / packed, m = q - kvh * packed, tok = a.group.div(m);
-            merge_one<T>(p, a.few_part, a.few_lse, a.few_parts, a.few_splits, ((long long)i * p.pages.kv_heads + kvh) * kFewRows + m, r0 + tok, kvh * G + m - tok * G,
-                         4 * (x - q * quads));
-        }
-        return;
-    }
-    const int lane = threadIdx.x & 63, row = blockIdx.x - request_blocks;
+    const int quads = p.pages.head_dim / 4;
+    const int lane = threadIdx.x & 63, row = blockIdx.x;
     // the request that owns the row: the last i with cu_rows[i] <= row
     int i = 0, span = p.requests;
     while (span > 1) {
@@ -856,11 +820,11 @@ __global__ __launch_bounds__(256) void attention_merge_kernel(AttnArgs a, unsign
         span = left < step ? left : step;
     }
     const int r0 = p.cu_rows[i], r1 = p.cu_rows[i + 1];
-    if (r0 < 0 || r0 > row || row >= r1 || r1 > p.rows || (long long)(r1 - r0) * G <= a.small) return;
+    if (r0 < 0 || r0 > row || row >= r1 || r1 > p.rows) return;
     const int x = blockIdx.y * 256 + threadIdx.x;
     if (x < p.q_heads * quads) {
         const int head = x / quads;
-        merge_one<T>(p, row_part, row_lse, row_parts, row_splits, (long long)row * p.q_heads + head, row, head, 4 * (x - head * quads));
+        merge_one<T>(a, row, head, 4 * (x - head * quads));
     }
 }
 
@@ -877,33 +841,17 @@ Cut cut_of(const PttsPagedAttention& p, int cus) {
     long long keys = std::max(1ll, static_cast<long long>(p.table_width) * p.pages.page_size);
     if (p.max_kv > 0) keys = std::min<long long>(keys, p.max_kv);
     if (p.window > 0) keys = std::min<long long>(keys, static_cast<long long>(p.window) + p.sinks + most_rows);  // what a tile sees
-    c.few = is_float || p.requests > 1 || most_rows * G <= kFewRows;
     c.chunk = !is_float && most_rows * G > kFewRows;
-    if (c.few && c.chunk) c.small = kFewRows;
-    c.chunk_tiles = packed / kChunkRows + p.requests;
-    c.few_tiles = c.small ? p.requests : packed / kFewRows + p.requests;
-    // Splits cost a second launch and a round trip of the rows, so they have to pay: they are made where the tiles alone leave
-    // compute units idle, and no split is shorter than what one workgroup reads in about that time.
-    auto splits = [&](long long groups, long long want, long long least_keys) {
-        const long long s = std::min(want / groups, keys / least_keys);
-        return static_cast<int>(std::max(1ll, std::min<long long>(s, kMostSplits)));
-    };
-    if (c.chunk) {
-        const long long groups = std::max(1ll, packed / kChunkRows) * kvh;
-        c.chunk_splits = splits(groups, 2ll * cus, 1024);
-        c.chunk_least = static_cast<int>(std::max(1ll, (keys / kChunkKeys + c.chunk_splits - 1) / c.chunk_splits));
-        c.chunk_parts = static_cast<long long>(p.rows) * p.q_heads;
-    }
-    if (c.few) {
-        const int step = is_float ? 64 : 128;          // keys of one step of a workgroup
-        const long long groups = std::max<long long>(p.requests, c.small ? 0 : packed / kFewRows) * kvh;
-        const long long resident = p.pages.head_dim <= 64 ? 3 : p.pages.head_dim <= 128 ? 2 : 1;       // workgroups of a compute unit
-        c.few_splits = splits(groups, resident * cus, c.small ? 4096 : (256 << 10) / (2 * p.pages.head_dim * type_size(p.pages.type)));
-        c.few_least = static_cast<int>(std::max(1ll, (keys / step + c.few_splits - 1) / c.few_splits));
-        c.few_parts = c.small ? static_cast<long long>(p.requests) * kvh * kFewRows : static_cast<long long>(p.rows) * p.q_heads;
-    }
-    const long long parts = (c.chunk_splits > 1 ? c.chunk_splits * c.chunk_parts : 0) + (c.few_splits > 1 ? c.few_splits * c.few_parts : 0);
-    c.bytes = parts * (p.pages.head_dim + 1ll) * 4;
+    const int rows = c.chunk ? kChunkRows : kFewRows;
+    c.tiles = packed / rows + p.requests;
+    const long long want = (c.chunk ? 2 : p.pages.head_dim <= 64 ? 3 : p.pages.head_dim <= 128 ? 2 : 1) * static_cast<long long>(cus);
+    const long long groups = std::max<long long>(p.requests, packed / rows) * kvh;
+    const long long least_keys = c.chunk ? 256 : (256 << 10) / (2 * p.pages.head_dim * type_size(p.pages.type));
+    c.splits = static_cast<int>(std::max(1ll, std::min({want / groups, keys / least_keys, static_cast<long long>(kMostSplits)})));
+    const int step = c.chunk ? kChunkKeys : is_float ? 64 : 128;          // keys of a block, of one step of a workgroup
+    c.least = static_cast<int>(std::max(1ll, (keys / step + c.splits - 1) / c.splits));
+    c.parts = static_cast<long long>(p.rows) * p.q_heads;
+    c.bytes = c.splits > 1 ? c.splits * c.parts * (p.pages.head_dim + 1ll) * 4 : 0;
     return c;
 }
 
@@ -917,16 +865,11 @@ template <typename T, typename C> void launch_few(const AttnArgs& a, unsigned gr
     else if (d <= 128) launch_few_of<T, C, 128>(a, grid, s);
     else launch_few_of<T, C, 256>(a, grid, s);
 }
-template <typename T, int DH> void launch_chunk_of(const AttnArgs& a, unsigned grid, hipStream_t s) {
-    if (a.few_blocks == 0) hipLaunchKernelGGL((attention_chunk_kernel<T, DH>), dim3(grid), dim3(256), 0, s, a);
-    else if (a.p.pages.head_dim == DH) hipLaunchKernelGGL((attention_both_kernel<T, DH, true>), dim3(grid), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((attention_both_kernel<T, DH, false>), dim3(grid), dim3(256), 0, s, a);
-}
 template <typename T> void launch_chunk(const AttnArgs& a, unsigned grid, hipStream_t s) {
     const int d = a.p.pages.head_dim;
-    if (d <= 64) launch_chunk_of<T, 64>(a, grid, s);
-    else if (d <= 128) launch_chunk_of<T, 128>(a, grid, s);
-    else launch_chunk_of<T, 256>(a, grid, s);
+    if (d <= 64) hipLaunchKernelGGL((attention_chunk_kernel<T, 64>), dim3(grid), dim3(256), 0, s, a);
+    else if (d <= 128) hipLaunchKernelGGL((attention_chunk_kernel<T, 128>), dim3(grid), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((attention_chunk_kernel<T, 256>), dim3(grid), dim3(256), 0, s, a);
 }
 
 unsigned grid_of(long long n) {
@@ -973,25 +916,19 @@ void launch_paged_attention(const PttsPagedAttention& p, int cus, hipStream_t s)
             throw std::runtime_error("paged_attention: a workspace of " + std::to_string(c.bytes) + " bytes is required");
         if (reinterpret_cast<uintptr_t>(p.workspace) % 16) throw std::runtime_error("paged_attention: the workspace must be aligned to 16 bytes");
     }
-    const long long few_blocks = c.few ? c.few_tiles * c.few_splits * p.pages.kv_heads : 0;
-    const unsigned grid = grid_of(few_blocks + (c.chunk ? c.chunk_tiles * c.chunk_splits * p.pages.kv_heads : 0));
+    const unsigned grid = grid_of(c.tiles * c.splits * p.pages.kv_heads);
     AttnArgs a;
     a.p = p;
     if (p.window > 1 << 30) a.p.window = 0;          // no context is that long
     a.page = FastDiv::of(static_cast<unsigned>(p.pages.page_size));
     a.group = FastDiv::of(static_cast<unsigned>(p.q_heads / p.pages.kv_heads));
     a.scale2 = p.scale * 1.4426950408889634f;
-    a.small = c.small;
-    a.few_blocks = static_cast<unsigned>(few_blocks);
-    a.chunk_tiles = c.chunk_tiles;
-    a.chunk_splits = c.chunk_splits; a.few_splits = c.few_splits;
-    a.chunk_least = c.chunk_least; a.few_least = c.few_least;
-    a.chunk_parts = c.chunk_parts; a.few_parts = c.few_parts;
-    const long long dim = p.pages.head_dim, chunk_rows = c.chunk_splits > 1 ? c.chunk_splits * c.chunk_parts : 0, few_rows = c.few_splits > 1 ? c.few_splits * c.few_parts : 0;
-    a.chunk_part = static_cast<float*>(p.workspace);
-    a.few_part = a.chunk_part + chunk_rows * dim;
-    a.chunk_lse = a.few_part + few_rows * dim;
-    a.few_lse = a.chunk_lse + chunk_rows;
+    a.tiles = c.tiles;
+    a.splits = c.splits;
+    a.least = c.least;
+    a.part = static_cast<float*>(p.workspace);
+    a.lse = a.part + c.splits * c.parts * p.pages.head_dim;
+    a.parts = c.parts;
     if (c.chunk) {
         if (p.q_type == PTTS_TYPE_BF16) launch_chunk<__bf16>(a, grid, s);
         else launch_chunk<_Float16>(a, grid, s);
@@ -1005,17 +942,11 @@ void launch_paged_attention(const PttsPagedAttention& p, int cus, hipStream_t s)
         launch_few<_Float16, _Float16>(a, grid, s);
     }
     if (c.bytes > 0) {
-        const bool rows_cut = c.chunk ? c.chunk_splits > 1 : true;
-        const unsigned requests = c.small && c.few_splits > 1 ? p.requests : 0;
-        // a request of the few form has at most kFewRows packed rows for each key head, a row q_heads
-        const long long items = std::max<long long>(rows_cut ? p.q_heads : 0, requests ? kFewRows * p.pages.kv_heads : 0) * (p.pages.head_dim / 4);
-        const dim3 merge(grid_of(requests + (rows_cut ? static_cast<long long>(p.rows) : 0)), static_cast<unsigned>((items + 255) / 256));
-        const int splits = c.chunk ? c.chunk_splits : c.few_splits;
-        const float *part = c.chunk ? a.chunk_part : a.few_part, *lse = c.chunk ? a.chunk_lse : a.few_lse;
-        const long long parts = c.chunk ? c.chunk_parts : c.few_parts;
-        if (p.q_type == PTTS_TYPE_F32) hipLaunchKernelGGL(attention_merge_kernel<float>, merge, dim3(256), 0, s, a, requests, splits, part, lse, parts);
-        else if (p.q_type == PTTS_TYPE_BF16) hipLaunchKernelGGL(attention_merge_kernel<__bf16>, merge, dim3(256), 0, s, a, requests, splits, part, lse, parts);
-        else hipLaunchKernelGGL(attention_merge_kernel<_Float16>, merge, dim3(256), 0, s, a, requests, splits, part, lse, parts);
+        const long long items = static_cast<long long>(p.q_heads) * (p.pages.head_dim / 4);
+        const dim3 merge(p.rows, static_cast<unsigned>((items + 255) / 256));
+        if (p.q_type == PTTS_TYPE_F32) hipLaunchKernelGGL(attention_merge_kernel<float>, merge, dim3(256), 0, s, a);
+        else if (p.q_type == PTTS_TYPE_BF16) hipLaunchKernelGGL(attention_merge_kernel<__bf16>, merge, dim3(256), 0, s, a);
+        else hipLaunchKernelGGL(attention_merge_kernel<_Float16>, merge, dim3(256), 0, s, a);
     }
 }
 

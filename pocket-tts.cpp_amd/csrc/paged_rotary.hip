@@ -2,7 +2,7 @@
 //
 // (a, b) -> (a cos - b sin, b cos + a sin) for each pair of a head.  The angle positions[row] * freq[i] is formed in float64 and
 // reduced to a fraction of a turn there, so that a position of a million loses nothing; sine and cosine of the fraction are
-// float32.  They depend on (row, pair) alone: a workgroup computes them once for its rows into LDS and then streams all heads past
+// float32.  They depend on (row, pair) alone: a workgroup computes them once for its row into LDS and then streams all heads past
 // them, which leaves the kernel at one read and one write of q, k and v.
 #include <algorithm>
 #include <cmath>
@@ -18,7 +18,6 @@ namespace {
 struct RotaryArgs {
     PttsRotaryAppend p;
     FastDiv page;
-    int group;       // rows per workgroup
     int units;       // work units of one row: rotated heads (q, k) times units per head, then v
     FastDiv per_head, per_v;   // units of a rotated head, of a value head
 };
@@ -57,47 +56,44 @@ template <typename T, int N, bool kStream> __device__ __forceinline__ void store
 // their partners in the second.  Interleaved: a unit is N (at least 2) neighbouring values, N / 2 pairs.
 template <typename T, typename C, int N, bool INTER, bool kStream>
 __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
-    extern __shared__ float2 turn[];                     // [group][rot_dim / 2]
-    __shared__ long long filed[2];                      // element offset of the row's slot in the pages, -1: none
+    __shared__ float2 turn[128];                         // [rot_dim / 2]
+    __shared__ long long place;                          // element offset of the row's slot in the pages, -1: none
     const PttsRotaryAppend& p = a.p;
     const int tid = threadIdx.x, half = p.rot_dim >> 1;
-    const int r0 = blockIdx.x * a.group, nr = p.rows - r0 < a.group ? p.rows - r0 : a.group;
-    if (tid < nr) {
+    const int row = blockIdx.x;
+    if (tid == 0) {
         long long at = -1;
         if (p.k) {
-            const int slot = p.slot_map[r0 + tid];
+            const int slot = p.slot_map[row];
             const unsigned pg = slot < 0 ? 0 : a.page.div(slot);
             if (slot >= 0 && pg < (unsigned)p.pages.pages)
                 at = (long long)pg * p.pages.page_stride + (long long)(slot - (int)pg * p.pages.page_size) * p.pages.row_stride;
             else if (slot != -1 && p.status) atomicOr(p.status, kStatusPage);
         }
-        filed[tid] = at;
+        place = at;
     }
-    for (int u = tid; u < nr * half; u += 256) {
-        const int r = u / half, i = u - r * half;
-        const double t = (double)p.positions[r0 + r] * (p.freq[i] * 0.15915494309189533577);   // turns
+    if (tid < half) {
+        const double t = (double)p.positions[row] * (p.freq[tid] * 0.15915494309189533577);   // turns
         float s, c;
         sincospif(2.0f * (float)(t - rint(t)), &s, &c);
-        turn[u] = make_float2(c * p.magnitude, s * p.magnitude);
+        turn[tid] = make_float2(c * p.magnitude, s * p.magnitude);
     }
     __syncthreads();
     constexpr int NN = INTER && N == 1 ? 2 : N;          // values of a unit outside the halves layout
     const int rot_heads = (p.q ? p.q_heads : 0) + (p.k ? p.pages.kv_heads : 0), q_heads = p.q ? p.q_heads : 0;
     const int turn_units = INTER ? p.rot_dim / NN : half / N;
-    const int total = nr * a.units;
-    for (int u = blockIdx.y * 256 + tid; u < total; u += gridDim.y * 256) {
-        const int r = u / a.units;
-        int w = u - r * a.units;
-        const long long row = r0 + r;
+    const long long filed = place;
+    for (int u = blockIdx.y * 256 + tid; u < a.units; u += gridDim.y * 256) {
+        int w = u;
         const int n_rot = rot_heads * (int)a.per_head.d;
         if (w < n_rot) {
             const int h = (int)a.per_head.div(w), e = w - h * (int)a.per_head.d;
             const bool is_q = h < q_heads;
-            if (!is_q && filed[r] < 0) continue;
-            const T* src = is_q ? (const T*)p.q + row * p.q_row_stride + (long long)h * p.q_head_stride
-                                : (const T*)p.k + row * p.k_row_stride + (long long)(h - q_heads) * p.k_head_stride;
-            T* qd = (T*)p.q_out + row * p.out_row_stride + (long long)h * p.out_head_stride;
-            C* kd = is_q ? nullptr : (C*)p.pages.k + filed[r] + (long long)(h - q_heads) * p.pages.head_stride;
+            if (!is_q && filed < 0) continue;
+            const T* src = is_q ? (const T*)p.q + (long long)row * p.q_row_stride + (long long)h * p.q_head_stride
+                                : (const T*)p.k + (long long)row * p.k_row_stride + (long long)(h - q_heads) * p.k_head_stride;
+            T* qd = (T*)p.q_out + (long long)row * p.out_row_stride + (long long)h * p.out_head_stride;
+            C* kd = is_q ? nullptr : (C*)p.pages.k + filed + (long long)(h - q_heads) * p.pages.head_stride;
             if (e >= turn_units) {                       // behind the rotated part
                 const int d0 = p.rot_dim + (e - turn_units) * NN;
                 float x[NN];
@@ -110,7 +106,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
                 load_f<T, NN, kStream>(src + d0, x);
 #pragma unroll
                 for (int i = 0; i < NN / 2; ++i) {
-                    const float2 cs = turn[r * half + d0 / 2 + i];
+                    const float2 cs = turn[d0 / 2 + i];
                     y[2 * i] = x[2 * i] * cs.x - x[2 * i + 1] * cs.y;
                     y[2 * i + 1] = x[2 * i + 1] * cs.x + x[2 * i] * cs.y;
                 }
@@ -123,7 +119,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
                 load_f<T, N, kStream>(src + half + d0, x1);
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
-                    const float2 cs = turn[r * half + d0 + i];
+                    const float2 cs = turn[d0 + i];
                     y0[i] = x0[i] * cs.x - x1[i] * cs.y;
                     y1[i] = x1[i] * cs.x + x0[i] * cs.y;
                 }
@@ -133,10 +129,10 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
         } else {
             w -= n_rot;
             const int h = (int)a.per_v.div(w), d0 = (w - h * (int)a.per_v.d) * NN;
-            if (filed[r] < 0) continue;
+            if (filed < 0) continue;
             float x[NN];
-            load_f<T, NN, kStream>((const T*)p.v + row * p.v_row_stride + (long long)h * p.v_head_stride + d0, x);
-            store_f<C, NN, kStream>((C*)p.pages.v + filed[r] + (long long)h * p.pages.head_stride + d0, x);
+            load_f<T, NN, kStream>((const T*)p.v + (long long)row * p.v_row_stride + (long long)h * p.v_head_stride + d0, x);
+            store_f<C, NN, kStream>((C*)p.pages.v + filed + (long long)h * p.pages.head_stride + d0, x);
         }
     }
 }
@@ -152,22 +148,21 @@ void dispatch(RotaryArgs a, bool wide, hipStream_t s) {
     a.per_head = FastDiv::of(static_cast<unsigned>(per_head));
     a.per_v = FastDiv::of(static_cast<unsigned>(per_v));
     a.units = rot_heads * per_head + (p.k ? p.pages.kv_heads * per_v : 0);
-    a.group = p.rows >= 2048 ? 2 : 1;
-    const dim3 grid((p.rows + a.group - 1) / a.group, std::min(4, std::max(1, 256 / p.rows))), block(256);
-    const size_t lds = static_cast<size_t>(a.group) * half * sizeof(float2);
+    // One row a workgroup (two took 37.9 us in place of 34.6 for the 8192 rows below), and up to four workgroups a row where rows are few.
+    const dim3 grid(p.rows, std::min(4, std::max(1, 256 / p.rows))), block(256);
     // What is more than the L2 caches hold between them (8 x 4 MB) cannot wait there for its reader, and passing it through them costs:
-    // 8192 rows of 48 heads of 128 in bf16 (201 MB) take 46.2 us through the caches and 37.7 us past them.  Smaller calls stay in
+    // 8192 rows of 48 heads of 128 in bf16 (201 MB) take 41.9 us through the caches and 34.6 us past them (5.8 TB/s).  Smaller calls stay in
     // the caches, where the attention that follows finds them.
     const long long moved = static_cast<long long>(p.rows) * p.pages.head_dim * ((p.q ? 2ll * p.q_heads * sizeof(T) : 0) + (p.k ? 2ll * p.pages.kv_heads * (sizeof(T) + sizeof(C)) : 0));
     const bool stream = moved > 32ll << 20;
     if (wide) {
-        if (p.interleaved && stream) hipLaunchKernelGGL((rotary_kernel<T, C, W, true, true>), grid, block, lds, s, a);
-        else if (p.interleaved) hipLaunchKernelGGL((rotary_kernel<T, C, W, true, false>), grid, block, lds, s, a);
-        else if (stream) hipLaunchKernelGGL((rotary_kernel<T, C, W, false, true>), grid, block, lds, s, a);
-        else hipLaunchKernelGGL((rotary_kernel<T, C, W, false, false>), grid, block, lds, s, a);
+        if (p.interleaved && stream) hipLaunchKernelGGL((rotary_kernel<T, C, W, true, true>), grid, block, 0, s, a);
+        else if (p.interleaved) hipLaunchKernelGGL((rotary_kernel<T, C, W, true, false>), grid, block, 0, s, a);
+        else if (stream) hipLaunchKernelGGL((rotary_kernel<T, C, W, false, true>), grid, block, 0, s, a);
+        else hipLaunchKernelGGL((rotary_kernel<T, C, W, false, false>), grid, block, 0, s, a);
     } else {
-        if (p.interleaved) hipLaunchKernelGGL((rotary_kernel<T, C, 1, true, false>), grid, block, lds, s, a);
-        else hipLaunchKernelGGL((rotary_kernel<T, C, 1, false, false>), grid, block, lds, s, a);
+        if (p.interleaved) hipLaunchKernelGGL((rotary_kernel<T, C, 1, true, false>), grid, block, 0, s, a);
+        else hipLaunchKernelGGL((rotary_kernel<T, C, 1, false, false>), grid, block, 0, s, a);
     }
 }
 
