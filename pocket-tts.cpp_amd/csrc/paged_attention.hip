@@ -841,10 +841,18 @@ Cut cut_of(const PttsPagedAttention& p, int cus) {
     long long keys = std::max(1ll, static_cast<long long>(p.table_width) * p.pages.page_size);
     if (p.max_kv > 0) keys = std::min<long long>(keys, p.max_kv);
     if (p.window > 0) keys = std::min<long long>(keys, static_cast<long long>(p.window) + p.sinks + most_rows);  // what a tile sees
-    c.chunk = !is_float && most_rows * G > kFewRows;
+    // Float rows have the few form alone.  Others take it where one workgroup a unit and a few of its longer steps do the whole call, that is where
+    // latency is all: one row of 16 heads of 64 on 200 keys takes 6.2 us and 9.2 in the chunk form, one of 16 / 2 heads of 128 on 600 keys
+    // 12.4 and 13.8; on 2048 keys the first takes 13.2 and 12.1, 64 such rows on 1024 keys 65 and 61, 16 rows of 16 / 2 heads of 128 on
+    // 4096 keys 30 and 23, 16 of 32 / 8 heads on 16384 keys 144 and 138, four rows a request 33 and 25.
+    c.chunk = !is_float && (most_rows * G > kFewRows || keys > 1024 || static_cast<long long>(p.requests) * kvh > cus);
     const int rows = c.chunk ? kChunkRows : kFewRows;
     c.tiles = packed / rows + p.requests;
-    const long long want = (c.chunk ? 2 : p.pages.head_dim <= 64 ? 3 : p.pages.head_dim <= 128 ? 2 : 1) * static_cast<long long>(cus);
+    // Splits cost a second launch and a round trip of the rows.  They are made up to what the compute units hold at once (24
+    // requests of one row, 16 heads of 64, about 1000 keys in a window: two a unit 30.2 us, three 26.1; heads of 128: 256 rows on 16384 keys without
+    // splits 351 us, one a unit 62, two 53, three 65), and none is shorter than what pays for the rest: 256 keys in the chunk form (16 requests of 4 rows on 4096
+    // keys: 128 keys 35 us, 256 28, 512 29, 1024 39), 256 KB of keys and values in the few form.
+    const long long want = (p.pages.head_dim <= 64 ? 3 : p.pages.head_dim <= 128 ? 2 : 1) * static_cast<long long>(cus);
     const long long groups = std::max<long long>(p.requests, packed / rows) * kvh;
     const long long least_keys = c.chunk ? 256 : (256 << 10) / (2 * p.pages.head_dim * type_size(p.pages.type));
     c.splits = static_cast<int>(std::max(1ll, std::min({want / groups, keys / least_keys, static_cast<long long>(kMostSplits)})));
