@@ -4,9 +4,15 @@
 // row m / G under head m % G.  Two forms work on tiles of packed rows:
 //
 //   chunk   128 packed rows, four waves of 32; key blocks of 64 go through LDS and are read by all four waves
-//   few     16 packed rows; four waves walk different keys straight from memory and join at the end (single tokens: bound by
-//           the one read of the keys and values)
+//   few     16 packed rows; four waves walk different keys straight from memory and join at the end (float rows, and the
+//           smallest calls, where its steps of 128 keys make the shorter chain)
 //   merge   joins the results of rows whose keys were cut into splits
+//
+// The work is 4 head_dim operations a visible (query, key) pair and head against 4 head_dim bytes (16 bit) a key and key head, so a chunk
+// is bound by the matrix pipes and the exponentials, single rows by the one read of the keys and values, short calls by the chain
+// of dependent reads (lengths, page ids, rows).  Measured: 2048 rows on 16384 keys, 32 / 8 heads of 128, bf16: 509 us, 1.01 PFLOP/s (a
+// library product of 8192^3 reaches 1.21); 16 rows on up to 16384 keys each, same heads, f16: 682 MB in 138 us, 4.9 TB/s (the
+// same reads alone 6.0, a large copy 5.1); 64 rows on about 594 keys, 16 heads of 64: 102 MB in 26 us; one float row on 218 keys 8 us.
 //
 // All products are formed transposed, S^T = K Q^T and O^T = V^T P^T, so that a lane keeps one query for the whole kernel (its
 // running maximum and sum are scalars of the lane) and the weights leave the first product in the layout the second one takes
@@ -226,7 +232,10 @@ __device__ __forceinline__ void copy16(const void* from, void* to) {
     __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) unsigned*)from, (__attribute__((address_space(3))) unsigned*)to, 16, 0, 0);
 }
 
-// Three workgroups per CU where the head fits (170 registers), else two or one.
+// 128 rows a workgroup: each block of keys is read from LDS by four waves, and two (heads of 128) to four workgroups share a unit, so that
+// one's exponentials run beside another's products.  The next block comes by asynchronous copies into the other LDS buffer; passing it through
+// registers took 638 us in place of 588 (2048 rows on 16384 keys, at that stage), three buffers 780, the next block's scores beside
+// this one's weights 650.
 template <typename T, int DH> __global__ __launch_bounds__(256, DH == 256 ? 1 : DH == 128 ? 2 : 3) void attention_chunk_kernel(AttnArgs a) {
     __shared__ __attribute__((aligned(16))) ChunkLds<T, DH> lds;
     const unsigned block = blockIdx.x;
@@ -361,7 +370,7 @@ template <typename T, int DH> __global__ __launch_bounds__(256, DH == 256 ? 1 : 
         for (int i = 0; i < KS - 3; ++i) { __builtin_amdgcn_sched_group_barrier(0x8, 2, 0); __builtin_amdgcn_sched_group_barrier(0x100, 2, 0); }
         __builtin_amdgcn_sched_group_barrier(0x8, 6, 0);
         // From here to the end of the block this wave goes first: two waves of a unit that run in step would otherwise form scores together
-        // and weights together, each waiting for the same pipe (chunk of 2048 rows on 16384 keys 598 -> 545 us).
+        // and weights together, each waiting for the same pipe (2048 rows on 16384 keys: 598 us without, 530 with it).
         __builtin_amdgcn_s_setprio(1);
         // lane: query col; s[b][r] belongs to key k0 + 32 b + 8 (r / 4) + 4 h + r % 4
         if (border) {
@@ -464,6 +473,9 @@ template <typename T, int DH> __global__ __launch_bounds__(256, DH == 256 ? 1 : 
 
 // ------------------------------------------------------------------ few
 
+// Bound by the chain of reads: rows are asked for one step ahead and page ids three, which took 16 rows on 16384 keys from 169 to 150 us
+// against reads at their use.
+//
 // Fragments of one step of a wave, straight from memory: NA blocks of 16 keys.  Keys: lane (row lane % 16, quarter g = lane / 16) reads
 // the units g of its row.  Values: the lane reads head values CPL m .. CPL m + CPL - 1 (m = lane % 16) of the rows 4 g + r, so that
 // column t of every lane forms the operand of output tile t; the output's order is then CPL * (its row) + t.
@@ -785,7 +797,8 @@ __device__ __forceinline__ void merge_some(const float* part, const float* lse, 
         }
 }
 
-// out = sum over splits of exp2(lse_s - lse) part_s, four values a thread.
+// out = sum over splits of exp2(lse_s - lse) part_s, four values a thread.  A chain of reads: 16 splits at a time, with four, a call of one row on
+// 32768 keys in 64 splits took 27.2 us in place of 22.
 template <typename T>
 __device__ __forceinline__ void merge_one(const AttnArgs& a, long long row, int head, int d) {
     const PttsPagedAttention& p = a.p;
