@@ -210,7 +210,7 @@ POCKET_TTS_API int ptts_rotary_frequencies(int rot_dim, double base, int scaling
 /* Rotates the first rot_dim values of every head of q and k by positions[row] * freq[i] (device, float64: far positions keep their
  * angle), pairs (2 i, 2 i + 1) if interleaved, else (i, i + rot_dim / 2), times `magnitude`; the rest of the head passes unscaled.  q goes to q_out (q itself
  * is allowed, with the same strides).  k and v go to the pages, row r to slot slot_map[r] (-1: not stored).  Two rows must not
- * name one slot.  q, or k and v (then pages and slot_map too), may be NULL.  q, q_out, k and v have `type`; the pages
+ * name one slot; rows < 2^24.  q, or k and v (then pages and slot_map too), may be NULL.  q, q_out, k and v have `type`; the pages
  * have the same, or bf16 under f32 rows (rounded to nearest even). */
 typedef struct {
     const void* q;

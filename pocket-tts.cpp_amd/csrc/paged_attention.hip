@@ -893,8 +893,9 @@ template <typename T> void launch_chunk(const AttnArgs& a, unsigned grid, hipStr
     else hipLaunchKernelGGL((attention_chunk_kernel<T, 256>), dim3(grid), dim3(256), 0, s, a);
 }
 
+// A launch holds fewer than 2^32 threads.
 unsigned grid_of(long long n) {
-    if (n > 0x7fffffffll) throw std::runtime_error("paged_attention: too many rows and heads for one call");
+    if (n >= 1 << 24) throw std::runtime_error("paged_attention: too many rows and heads for one call");
     return static_cast<unsigned>(n);
 }
 

@@ -7,6 +7,7 @@ library (the first call here does it too).
 
 Every call enqueues on `stream` (a torch stream or a handle; default: torch's current stream of the tensors' device, the default
 stream for DeviceArray) and returns without waiting.  Nothing is kept between calls.  Failures raise ptts_lib.PttsError.
+For inference: nothing is recorded for torch's autograd.
 """
 from __future__ import annotations
 

@@ -113,6 +113,12 @@ def test_attention_refuses_what_passes_31_bits():
         _attention(**many)
 
 
+def test_rotary_refuses_more_threads_than_a_launch_holds():
+    n = 1 << 24
+    with pytest.raises(ptts_lib.PttsError, match="2\\^24"):
+        ptts_paged.rotary_append(arr((n, 1, 8), "float32"), None, None, arr((n,)), arr((4,), "float64"))
+
+
 def test_null_arguments():
     L = ptts_lib.load()
     assert L.ptts_paged_plan(None, 0, None) == -1

@@ -354,6 +354,21 @@ def test_torch_tensors(tmp_path):
     assert r.stdout.count("refused:") == 6
 
 
+def test_device_out_of_range_is_refused():
+    import ptts_lib
+    import ptts_paged
+    from ptts_paged import DeviceArray
+    a = {k: DeviceArray(1 << 20, (1,) if k != "t" else (1, 4), "int32", None, 99) for k in ("c", "n", "f", "t", "s", "p", "k")}
+    with pytest.raises(ptts_lib.PttsError, match="device 99"):
+        ptts_paged.plan(a["c"], a["n"], a["f"], a["t"], 16, slot_map=a["s"], positions=a["p"], cu_rows=DeviceArray(1 << 20, (2,), "int32", None, 99),
+                        kv_len=a["k"], counts=DeviceArray(1 << 20, (4,), "int32", None, 99))
+    loop = Loop()                                           # and the next call runs
+    loop.feed((1, 2, 3), np.random.default_rng(0))
+    _clear_slots(loop)
+    loop.launch()
+    loop.check()
+
+
 def _one_request(kind, q, k, v, new, splits_wanted=True):
     """Attention of the last `new` rows of one sequence, pages in order; returns out, lse."""
     import ptts_paged
