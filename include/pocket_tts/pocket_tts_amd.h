@@ -233,7 +233,7 @@ POCKET_TTS_API int ptts_rotary_append(const PttsRotaryAppend* args, int device, 
  * (window <= 0 or j > p - window or j < sinks).  out = softmax(scale q.k) v, lse (may be NULL) = ln sum exp(scale q.k); a row that
  * sees nothing gets 0 and -inf.  Head h of q reads head h / (q_heads / kv_heads) of the pages.  Keys that a row does not see
  * never reach it, whatever they hold.  out may not alias q.
- * Types: q and out q_type; pages of q_type, or bf16 pages under f32 rows.  Rows outside every request stay as they were.
+ * rows * (q_heads / kv_heads) < 2^30.  Types: q and out q_type; pages of q_type, or bf16 pages under f32 rows.  Rows outside every request stay as they were.
  * max_rows, max_kv: what the caller knows of the largest row count and length of a request (0: nothing).  They choose how the work
  * is cut and cost time when wrong, never results.
  * workspace: ptts_paged_attention_workspace() bytes (0: none needed; -1: bad arguments), 16-byte aligned, contents irrelevant
