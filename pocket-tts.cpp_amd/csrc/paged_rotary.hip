@@ -194,7 +194,7 @@ void check_rotary_append(const PttsRotaryAppend& p) {
     const char* who = "rotary_append";
     const std::string w = std::string(who) + ": ";
     if (p.rows < 0 || p.rows >= 1 << 24) throw std::runtime_error(w + "rows must be 0 to 2^24 - 1");
-    if (!p.q && !p.k) throw std::runtime_error(w + "nothing to rotate: q and k are both missing");
+    if (p.rows > 0 && !p.q && !p.k) throw std::runtime_error(w + "nothing to rotate: q and k are both missing");
     if (!p.k != !p.v) throw std::runtime_error(w + "k and v come together");
     if (p.type != PTTS_TYPE_F32 && p.type != PTTS_TYPE_BF16 && p.type != PTTS_TYPE_F16) throw std::runtime_error(w + "unknown type");
     if (p.k) {
