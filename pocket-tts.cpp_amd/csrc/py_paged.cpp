@@ -456,10 +456,10 @@ Names g_workspace_names = {"attention_workspace", 12, 6, 0x3f, {"q", "k_pages", 
 PyObject* attention_workspace(PyObject*, PyObject* const* args, Py_ssize_t nargs, PyObject* kwnames) {
     PyObject* o[12];
     if (!parse(g_workspace_names, args, nargs, kwnames, o)) return nullptr;
-    PyObject* full[14] = {o[0], o[1], o[2], o[3], o[4], o[5], o[6] ? o[6] : o[0], nullptr, o[7], o[8], o[9], o[10], o[11], nullptr};
+    PyObject* full[14] = {o[0], o[1], o[2], o[3], o[4], o[5], is_none(o[6]) ? o[0] : o[6], nullptr, o[7], o[8], o[9], o[10], o[11], nullptr};
     AttentionCall c;
     if (!attention_args(full, c)) return nullptr;
-    if (!o[6]) c.p.out = static_cast<char*>(c.p.out) + (c.p.out ? 16 : 0);      // stands for an out of its own, which is not looked at here
+    if (is_none(o[6])) c.p.out = static_cast<char*>(c.p.out) + (c.p.out ? 16 : 0);      // stands for an out of its own, which is not looked at here
     const long long need = g_lib.workspace(&c.p, c.first->device);
     if (need < 0) return ran(-1);
     return PyLong_FromLongLong(need);

@@ -31,3 +31,13 @@ def test_a_step_without_rows(parts):
     k = arr((0, 2, 64), "bfloat16") if "kv" in parts else None
     passes_checks(ptts_paged.rotary_append, q, k, k, arr((0,)), arr((32,), "float64"), **more)
     passes_checks(ptts_paged.attention, x, pages, pages, arr((3, 5)), arr((4,)), arr((3,)), out=x)
+
+
+def test_workspace_query_with_an_explicit_none():
+    """out=None is the documented default of the query."""
+    x, pages = arr((5, 4, 64), "bfloat16"), arr((9, 16, 2, 64), "bfloat16")
+    lead = (x, pages, pages, arr((3, 5)), arr((4,)), arr((3,)))
+    passes_checks(ptts_paged.attention_workspace, *lead)
+    passes_checks(ptts_paged.attention_workspace, *lead, out=None)
+    with pytest.raises(ptts_lib.PttsError, match="must not be q"):
+        ptts_paged.attention_workspace(*lead, out=x)
