@@ -1,0 +1,72 @@
+"""Paged LM states with a window and sinks against a float64 model that keeps every row, in pools that are exactly large enough, and
+what calls that are refused leave behind."""
+
+import numpy as np
+import pytest
+
+from lm_ref import Lm
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def eng(packs):
+    import ptts_lib
+    e = ptts_lib.Engine(packs["small"][0], precision="fp32", temperature=0.0, lsd_steps=2, max_frames=64)
+    yield e
+    e.close()
+
+
+def _rows(rng, n, d):
+    return (rng.standard_normal((n, d)) * 0.5).astype(np.float32)
+
+
+def _held(length, page, window, sinks):
+    """Pages of a slot of `length` rows after its last row went in alone: those of the sinks and those that this row's window touches."""
+    return sum(p * page < sinks or (p + 1) * page > length - window for p in range(-(-length // page))) if window else -(-length // page)
+
+
+@pytest.mark.parametrize("page,window,sinks", [(8, 40, 11), (8, 40, 16), (7, 33, 0), (1, 20, 3), (16, 16, 17), (5, 1, 0)])
+def test_window_in_a_pool_without_a_spare_page(eng, packs, page, window, sinks):
+    """Pages that fall behind the window are taken by the other slot in the same step, so a page given back too early, or a row of the sinks
+    lost, changes the results; the free pages say whether one is given back too late."""
+    _, spec, w = packs["small"]
+    rng = np.random.default_rng(page)
+    start, steps = (23, 9, 1), 90
+    length = np.array(start)
+    pool = max(sum(_held(n + k, page, window, sinks) for n in start) for k in range(1, steps + 1))
+    pool = max(pool, sum(-(-n // page) for n in start))
+    st, refs = eng.paged_state(3, pages=pool, page_size=page, max_context=200, window=window, sinks=sinks), [Lm(spec, w, window, sinks) for _ in start]
+    for i, n in enumerate(start):
+        x = _rows(rng, n, eng.d_model)
+        eng.lm_prefill(st, i, x)
+        refs[i].rows(x)
+    assert st.free_pages() == pool - sum(-(-n // page) for n in start)
+    seq = np.full((3, eng.latent), np.nan, np.float32)
+    for k in range(steps):
+        cond, eos = eng.lm_step(st, seq)
+        length += 1
+        assert st.free_pages() == pool - sum(_held(n, page, window, sinks) for n in length), k
+        for i, r in enumerate(refs):
+            want, want_eos = r.latent(seq[i])
+            # float32 sums of a few hundred terms in two layers, as against the oracle
+            assert np.abs(cond[i] - want).max() < 1e-3 and abs(eos[i] - want_eos) < 1e-3, (k, i)
+        seq = (rng.standard_normal((3, eng.latent)) * 0.7).astype(np.float32)
+    st.close()
+
+
+def test_window_over_prompts_in_chunks(eng, packs):
+    """Prompts longer than the window, in passes of 128 rows and in pieces, then steps."""
+    _, spec, w = packs["small"]
+    rng = np.random.default_rng(3)
+    st, ref = eng.paged_state(1, pages=22, page_size=16, max_context=600, window=100, sinks=20), Lm(spec, w, 100, 20)
+    for n in (300, 1, 77):
+        x = _rows(rng, n, eng.d_model)
+        eng.lm_prefill(st, 0, x)
+        ref.rows(x)
+    for k in range(4):
+        z = (rng.standard_normal((1, eng.latent)) * 0.7).astype(np.float32)
+        cond, eos = eng.lm_step(st, z)
+        want, want_eos = ref.latent(z[0])
+        assert np.abs(cond[0] - want).max() < 1e-3 and abs(eos[0] - want_eos) < 1e-3, k
+    st.close()
