@@ -14,7 +14,13 @@
 
 namespace ptts {
 
-PagedCache::PagedCache(const Spec& s, int slots, int kv16_, const PagedOptions& o) : opt(o), kv16(kv16_), layers(s.lm_layers), heads(s.lm_heads) {
+// Sinks beyond the context are the whole context; as such their page count stays inside an int.
+static PagedOptions within(PagedOptions o) {
+    o.sinks = std::min(o.sinks, o.max_context);
+    return o;
+}
+
+PagedCache::PagedCache(const Spec& s, int slots, int kv16_, const PagedOptions& o) : opt(within(o)), kv16(kv16_), layers(s.lm_layers), heads(s.lm_heads) {
     if (slots <= 0 || o.pages <= 0 || o.page_size <= 0 || o.max_context <= 0) throw std::runtime_error("slots, pages, page_size and max_context must be positive");
     if (static_cast<long long>(o.pages) * o.page_size >= 1ll << 30 || o.max_context >= 1 << 30) throw std::runtime_error("the pool must hold fewer than 2^30 rows");
     if (o.window < 0 || o.sinks < 0) throw std::runtime_error("window and sinks must not be negative");

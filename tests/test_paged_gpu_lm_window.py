@@ -70,3 +70,20 @@ def test_window_over_prompts_in_chunks(eng, packs):
         want, want_eos = ref.latent(z[0])
         assert np.abs(cond[0] - want).max() < 1e-3 and abs(eos[0] - want_eos) < 1e-3, k
     st.close()
+
+
+@pytest.mark.parametrize("sinks", [2 ** 31 - 1, 200])
+def test_sinks_that_cover_everything(eng, packs, sinks):
+    """With all rows sinks a window hides nothing and no page comes back."""
+    _, spec, w = packs["small"]
+    rng = np.random.default_rng(5)
+    st, ref = eng.paged_state(1, pages=9, page_size=8, max_context=72, window=5, sinks=sinks), Lm(spec, w)
+    x = _rows(rng, 30, eng.d_model)
+    eng.lm_prefill(st, 0, x)
+    ref.rows(x)
+    for k in range(40):
+        z = (rng.standard_normal((1, eng.latent)) * 0.7).astype(np.float32)
+        cond, _ = eng.lm_step(st, z)
+        assert np.abs(cond[0] - ref.latent(z[0])[0]).max() < 1e-3, k
+        assert st.free_pages() == 9 - -(-(31 + k) // 8)
+    st.close()
