@@ -167,7 +167,7 @@ public:
 private:
     void release(int page);
     void drop(int slot);
-    void drop_behind_window(int slot, int length);
+    template <typename F> void behind_window(int slot, int length, F&& take);
     int kv16, layers, heads, width = 0, most = 0, now_slot0 = 0, now_nb = 0, now_rows = 0;
     size_t layer_bytes = 0;
     DevBuf k, v, table, ints, freq, slot_map, positions, work;

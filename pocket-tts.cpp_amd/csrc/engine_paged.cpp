@@ -67,16 +67,13 @@ void PagedCache::release(int page) {
     if (page >= 0 && --uses[page] == 0) free_pages.push_back(page);
 }
 
-// Pages that no later row of the slot can see: behind the window and past the sinks.
-void PagedCache::drop_behind_window(int slot, int length) {
+// Pages of a slot that no row from position `length` on can see: behind the window and past the sinks.
+template <typename F> void PagedCache::behind_window(int slot, int length, F&& take) {
     if (opt.window == 0) return;
     const long long low = static_cast<long long>(length) - opt.window + 1;      // first key that the next row's window holds
     auto& h = held[slot];
     for (long long i = (opt.sinks + opt.page_size - 1) / opt.page_size; i < static_cast<long long>(h.size()) && (i + 1) * opt.page_size <= low; ++i)
-        if (h[i] >= 0) {
-            release(h[i]);
-            h[i] = -1;
-        }
+        if (h[i] >= 0) take(h[i]);
 }
 
 // Throws if `rows` new rows of a slot, taken `chunk` at a time, would run out of pages or of context; changes nothing.
@@ -94,15 +91,17 @@ void PagedCache::check_room(int slot, int length, int rows, int chunk) const {
     }
 }
 
-// Block table, slot map and positions of `rows` new rows of each slot slot0 .. slot0 + nb - 1, at the lengths `pos`.
+// Block table, slot map and positions of `rows` new rows of each slot slot0 .. slot0 + nb - 1, at the lengths `pos`.  Throws if they do
+// not fit, before anything changes.
 void PagedCache::plan(int slot0, int nb, int rows, const int* pos, hipStream_t st) {
-    int need = 0;
+    long long need = 0, back = 0;              // pages taken; pages that come back, those shared between these slots once
     for (int i = 0; i < nb; ++i) {
         if (pos[i] + static_cast<long long>(rows) > opt.max_context) throw std::runtime_error("LM context exceeds max_context");
-        drop_behind_window(slot0 + i, pos[i]);
         need += (pos[i] + rows + opt.page_size - 1) / opt.page_size - static_cast<int>(held[slot0 + i].size());
     }
-    if (need > static_cast<int>(free_pages.size()))
+    for (int i = 0; i < nb; ++i) behind_window(slot0 + i, pos[i], [&](int page) { back += --uses[page] == 0; });
+    for (int i = 0; i < nb; ++i) behind_window(slot0 + i, pos[i], [&](int page) { ++uses[page]; });
+    if (need > free_count() + back)
         throw std::runtime_error("the pool has " + std::to_string(free_pages.size()) + " free pages, " + std::to_string(need) + " are needed");
     if (slot_map.bytes < static_cast<size_t>(nb) * rows * 4) {
         PTTS_HIP(hipStreamSynchronize(st));
@@ -110,6 +109,11 @@ void PagedCache::plan(int slot0, int nb, int rows, const int* pos, hipStream_t s
         positions.alloc(static_cast<size_t>(nb) * rows * 4);
     }
     PTTS_HIP(hipStreamSynchronize(st));        // the last call's copies have left the pinned block
+    for (int i = 0; i < nb; ++i)
+        behind_window(slot0 + i, pos[i], [&](int& page) {
+            release(page);
+            page = -1;
+        });
     int taken = 0;
     most = 0;
     for (int i = 0; i < nb; ++i) {

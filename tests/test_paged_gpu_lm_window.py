@@ -87,3 +87,43 @@ def test_sinks_that_cover_everything(eng, packs, sinks):
         assert np.abs(cond[0] - ref.latent(z[0])[0]).max() < 1e-3, k
         assert st.free_pages() == 9 - -(-(31 + k) // 8)
     st.close()
+
+
+def test_refused_step_gives_no_page_back(eng):
+    """Three slots need a page each and one could give one back: the step is refused and the first rows can still be shared."""
+    import ptts_lib
+    rng = np.random.default_rng(6)
+    st = eng.paged_state(3, pages=4, page_size=8, max_context=64, window=8)
+    for i, n in enumerate((16, 8, 8)):
+        eng.lm_prefill(st, i, _rows(rng, n, eng.d_model))
+    assert st.free_pages() == 0
+    seq = np.zeros((3, eng.latent), np.float32)
+    with pytest.raises(ptts_lib.PttsError, match="free pages"):
+        eng.lm_step(st, seq)
+    assert st.free_pages() == 0
+    st.share(0, 1, 8)                       # page 0 of slot 0 is still there; slot 1's comes back
+    assert st.free_pages() == 1
+    st.close()
+    # the limit of the context is met by the second slot only
+    st = eng.paged_state(2, pages=20, page_size=8, max_context=24, window=8)
+    for i, n in enumerate((17, 24)):
+        eng.lm_prefill(st, i, _rows(rng, n, eng.d_model))
+    free = st.free_pages()
+    with pytest.raises(ptts_lib.PttsError, match="max_context"):
+        eng.lm_step(st, np.zeros((2, eng.latent), np.float32))
+    assert st.free_pages() == free
+    st.close()
+
+
+def test_step_that_fits_through_pages_shared_behind_the_window(eng):
+    """Two slots share the pages that both leave behind in one step: they come back once, and the step takes them."""
+    rng = np.random.default_rng(7)
+    st = eng.paged_state(2, pages=3, page_size=8, max_context=64, window=8)
+    eng.lm_prefill(st, 0, _rows(rng, 16, eng.d_model))
+    st.share(0, 1, 16)
+    assert st.free_pages() == 1             # 2 pages, both in both slots
+    seq = np.zeros((2, eng.latent), np.float32)
+    out = eng.lm_step(st, seq)[0]           # both give page 0 back and need one each
+    assert st.free_pages() == 0
+    np.testing.assert_array_equal(out[0], out[1])
+    st.close()
