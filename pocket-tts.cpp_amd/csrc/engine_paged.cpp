@@ -185,7 +185,8 @@ void PagedCache::share(int from, int to, int rows, int from_length, hipStream_t 
     const auto& f = held[from];
     for (int i = 0; i < used; ++i)
         if (f[i] < 0) throw std::runtime_error("rows behind the window have been given back");
-    if (rest && free_pages.empty()) throw std::runtime_error("the pool has no free page");
+    const bool own = std::any_of(held[to].begin(), held[to].end(), [&](int page) { return page >= 0 && uses[page] == 1; });   // come back below
+    if (rest && free_pages.empty() && !own) throw std::runtime_error("the pool has no free page");
     drop(to);
     auto& t = held[to];
     t.assign(f.begin(), f.begin() + whole);

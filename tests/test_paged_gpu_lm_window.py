@@ -127,3 +127,32 @@ def test_step_that_fits_through_pages_shared_behind_the_window(eng):
     assert st.free_pages() == 0
     np.testing.assert_array_equal(out[0], out[1])
     st.close()
+
+
+def test_share_into_a_slot_of_a_full_pool(eng, packs):
+    """A finished utterance's slot begins anew with the voice though no page is free: its own pages serve."""
+    import ptts_lib
+    _, spec, w = packs["small"]
+    rng = np.random.default_rng(8)
+    voice, other = _rows(rng, 11, eng.d_model), _rows(rng, 16, eng.d_model)
+    st, ref = eng.paged_state(2, pages=4, page_size=8, max_context=32), Lm(spec, w)
+    eng.lm_prefill(st, 0, voice)
+    eng.lm_prefill(st, 1, other)
+    assert st.free_pages() == 0
+    st.share(0, 1, 11)
+    assert st.free_pages() == 1             # the whole page is shared, the three rows of the second are copied
+    eng.lm_prefill(st, 1, other[:5])
+    ref.rows(voice)
+    ref.rows(other[:5])
+    z = np.zeros((2, eng.latent), np.float32)
+    cond, _ = eng.lm_step(st, z)
+    assert np.abs(cond[1] - ref.latent(z[1])[0]).max() < 1e-3
+    st.close()
+    # pages that are shared with the source do not serve
+    st = eng.paged_state(2, pages=2, page_size=8, max_context=32)
+    eng.lm_prefill(st, 0, _rows(rng, 11, eng.d_model))
+    st.share(0, 1, 8)
+    with pytest.raises(ptts_lib.PttsError, match="no free page"):
+        st.share(0, 1, 9)
+    assert st.free_pages() == 0
+    st.close()
