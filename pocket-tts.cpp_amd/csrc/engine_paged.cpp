@@ -103,11 +103,11 @@ void PagedCache::plan(int slot0, int nb, int rows, const int* pos, hipStream_t s
     for (int i = 0; i < nb; ++i) behind_window(slot0 + i, pos[i], [&](int page) { ++uses[page]; });
     if (need > free_count() + back)
         throw std::runtime_error("the pool has " + std::to_string(free_pages.size()) + " free pages, " + std::to_string(need) + " are needed");
-    if (slot_map.bytes < static_cast<size_t>(nb) * rows * 4) {
-        PTTS_HIP(hipStreamSynchronize(st));
-        slot_map.alloc(static_cast<size_t>(nb) * rows * 4);
-        positions.alloc(static_cast<size_t>(nb) * rows * 4);
-    }
+    for (DevBuf* b : {&slot_map, &positions})
+        if (b->bytes < static_cast<size_t>(nb) * rows * 4) {
+            PTTS_HIP(hipStreamSynchronize(st));
+            b->alloc(static_cast<size_t>(nb) * rows * 4);
+        }
     PTTS_HIP(hipStreamSynchronize(st));        // the last call's copies have left the pinned block
     for (int i = 0; i < nb; ++i)
         behind_window(slot0 + i, pos[i], [&](int& page) {
