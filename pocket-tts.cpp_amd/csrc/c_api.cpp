@@ -442,11 +442,7 @@ POCKET_TTS_API int ptts_state_share(PocketTTSHandle handle, void* state, int fro
 
 POCKET_TTS_API int ptts_state_free_pages(PocketTTSHandle handle, void* state) {
     if (!handle || !state) { set_error("Invalid parameters"); return -1; }
-    return guarded("state_free_pages: ", [&] {
-        const auto* b = static_cast<ptts::Batch*>(state);
-        if (!b->paged) throw std::runtime_error("the state was not created with pages");
-        return b->paged->free_count();
-    });
+    return guarded("state_free_pages: ", [&] { return tts_of(handle)->engine().op_state_free_pages(static_cast<ptts::Batch*>(state)); });
 }
 
 POCKET_TTS_API void ptts_state_free(PocketTTSHandle handle, void* state) {

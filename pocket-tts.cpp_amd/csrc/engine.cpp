@@ -937,7 +937,11 @@ Batch* Engine::batch_new(int B) {
     return new Batch(*this, B);
 }
 void Engine::batch_free(Batch* b) { delete b; }
-void Engine::batch_reset(Batch* b) { b->reset(stream_); }
+void Engine::batch_reset(Batch* b) {
+    std::lock_guard<std::mutex> guard(mu_);
+    PTTS_HIP(hipSetDevice(opt_.device));
+    b->reset(stream_);
+}
 
 Batch* Engine::acquire_batch(int B, int lane) {
     auto key = std::make_pair(B, lane);

@@ -250,6 +250,7 @@ public:
     Batch* batch_new(int B);
     Batch* batch_new_paged(int B, const PagedOptions& o);
     void op_state_share(Batch* b, int from, int to, int rows);
+    int op_state_free_pages(Batch* b);
     void batch_free(Batch* b);
     void batch_reset(Batch* b);
     void op_lm_prefill(Batch* b, int slot, const float* emb, int rows);

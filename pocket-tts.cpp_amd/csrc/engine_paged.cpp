@@ -223,6 +223,12 @@ Batch* Engine::batch_new_paged(int B, const PagedOptions& o) {
     return new Batch(*this, B, false, &o);
 }
 
+int Engine::op_state_free_pages(Batch* b) {
+    std::lock_guard<std::mutex> guard(mu_);
+    if (!b->paged) throw std::runtime_error("the state was not created with pages");
+    return b->paged->free_count();
+}
+
 void Engine::op_state_share(Batch* b, int from, int to, int rows) {
     std::lock_guard<std::mutex> guard(mu_);
     PTTS_HIP(hipSetDevice(opt_.device));

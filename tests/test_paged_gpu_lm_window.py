@@ -1,5 +1,6 @@
 """Paged LM states with a window and sinks against a float64 model that keeps every row, in pools that are exactly large enough, and
 what calls that are refused leave behind."""
+import threading
 
 import numpy as np
 import pytest
@@ -156,3 +157,29 @@ def test_share_into_a_slot_of_a_full_pool(eng, packs):
         st.share(0, 1, 9)
     assert st.free_pages() == 0
     st.close()
+
+
+def test_free_pages_and_reset_beside_steps(eng):
+    """Another thread asks for the free pages, and resets a state of its own, while steps run."""
+    a, b = (eng.paged_state(2, pages=40, page_size=2, max_context=40) for _ in range(2))
+    seen, stop, errors = set(), threading.Event(), []
+
+    def ask():
+        try:
+            while not stop.is_set():
+                seen.add(a.free_pages())
+                b.reset()
+        except BaseException as e:
+            errors.append(e)
+
+    t = threading.Thread(target=ask)
+    t.start()
+    try:
+        for _ in range(40):
+            eng.lm_step(a, np.zeros((2, eng.latent), np.float32))
+    finally:
+        stop.set()
+        t.join()
+    assert not errors and seen <= set(range(0, 41, 2)) and a.free_pages() == 0 and b.free_pages() == 40
+    a.close()
+    b.close()
