@@ -117,7 +117,13 @@ template <int kPer> __global__ __launch_bounds__(256) void plan_kernel(PlanArgs 
                 p.cu_rows[c0 + i0 + j] = (int)(r < 0x7fffffff ? r : 0x7fffffff);
                 p.kv_len[c0 + i0 + j] = cach[j] + arr[j];
             }
-            // rows of this request that end up without a page: those behind the last page that it holds or gets
+            // rows of this request that end up without a page: those of a held page that is missing (an earlier plan's -1), and those
+            // behind the last page that it holds or gets
+            const int full = (int)a.page.div(cach[j]);
+            if (full < hv[j] && arr[j] > 0 && old[j] < 0) {
+                const long long room = (full + 1ll) * ps - cach[j];
+                no_page += arr[j] < room ? arr[j] : room;
+            }
             const long long got = p.n_free - k < 0 ? 0 : p.n_free - k < need[j] ? p.n_free - k : need[j];
             const long long first_out = (hv[j] + got) * ps > cach[j] ? (hv[j] + got) * ps : cach[j];
             if (cach[j] + (long long)arr[j] > first_out) no_page += cach[j] + (long long)arr[j] - first_out;

@@ -1,0 +1,28 @@
+"""The paged-cache operators at the borders of what their documentation allows, through the public bindings."""
+import numpy as np
+import pytest
+
+import paged_ref as ref
+
+pytestmark = pytest.mark.gpu
+
+
+def test_plan_counts_rows_of_a_held_page_that_is_missing():
+    """A page that an earlier plan could not give: rows that still fall into it have no page, and are counted."""
+    from test_paged_gpu import _run_plan
+    table = np.array([[4, -1, -1, -1], [2, 3, -1, -1], [-1, -1, -1, -1]])
+    for cached, arriving in (([5, 6, 0], [2, 1, 3]), ([5, 6, 0], [9, 0, 0]), ([4, 8, 4], [1, 1, 0]), ([7, 3, 3], [1, 1, 1])):
+        free = np.arange(10, 20)
+        rows = sum(arriving)
+        want = ref.plan(cached, arriving, free, table, 4, rows)
+        got, status = _run_plan(cached, arriving, 4, table, free, rows)
+        for name, g, w in zip(("table", "slots", "positions", "cu", "kv_len", "counts"), got, want):
+            np.testing.assert_array_equal(g, w, err_msg=f"{name} {cached} {arriving}")
+        assert status == 0
+    many = 300                                             # the form for many requests
+    table = np.where(np.arange(many)[:, None] % 3 == 0, -1, np.arange(2 * many).reshape(many, 2))
+    cached, arriving = np.full(many, 2), np.arange(many) % 5
+    want = ref.plan(cached, arriving, np.arange(1000, 1500), table, 4, int(arriving.sum()))
+    got, _ = _run_plan(cached, arriving, 4, table, np.arange(1000, 1500), int(arriving.sum()))
+    for g, w in zip(got, want):
+        np.testing.assert_array_equal(g, w)
