@@ -180,7 +180,8 @@ typedef struct {
  * rows (request 0's first) gets positions[r] and slot_map[r] = page * page_size + row inside the page.  cu_rows[i] is the first
  * packed row of request i (requests + 1 entries), kv_len[i] = cached[i] + arriving[i].
  * counts[4] = new rows in all (those beyond `rows` are not written), pages taken, pages missing, rows without a page.  A page that is missing (free list exhausted, or
- * table row full) leaves -1 in the table and its rows get slot -1.  A negative length counts as 0.
+ * table row full) leaves -1 in the table and its rows get slot -1, in later plans too.  An id below 0 in free_pages is entered as it
+ * is and its rows get slot -1 (status 1; counts takes it for a page).  A negative length counts as 0.
  * Rows of slot_map and positions behind the last new row stay as they are.  The last page of a request must not be shared when
  * it is partly filled and rows arrive.  requests <= 65536. */
 typedef struct {

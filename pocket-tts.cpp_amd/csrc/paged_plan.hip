@@ -147,7 +147,9 @@ template <int kPer> __global__ __launch_bounds__(256) void plan_kernel(PlanArgs 
         const long long ka = k_lo > pick0[0] ? k_lo : pick0[0], kb = k_hi < pick0[n] ? k_hi : pick0[n];
         for (long long q = ka + tid; q < kb; q += 256) {
             const int i = find_last(pick0, n, q);
-            p.block_table[(long long)(c0 + i) * p.table_stride + have[i] + (int)(q - pick0[i])] = free_page(q);
+            const int id = free_page(q);
+            if (id < 0 && q < p.n_free) bad |= 2;
+            p.block_table[(long long)(c0 + i) * p.table_stride + have[i] + (int)(q - pick0[i])] = id;
         }
     }
     // totals, the same in every workgroup

@@ -26,3 +26,12 @@ def test_plan_counts_rows_of_a_held_page_that_is_missing():
     got, _ = _run_plan(cached, arriving, 4, table, np.arange(1000, 1500), int(arriving.sum()))
     for g, w in zip(got, want):
         np.testing.assert_array_equal(g, w)
+
+
+def test_plan_reports_free_pages_that_are_none():
+    """An id below 0 in the free list: the rows that fall into it get no slot and the status says so; one that no row needs does not matter."""
+    from test_paged_gpu import _run_plan
+    got, status = _run_plan([0, 0], [5, 3], 4, np.full((2, 3), -1), np.array([7, -3, 9, -1]), 8)
+    assert status == 1 and got[1].tolist() == [28, 29, 30, 31, -1, 36, 37, 38]
+    got, status = _run_plan([0, 0], [4, 3], 4, np.full((2, 3), -1), np.array([7, 9, -1]), 7)
+    assert status == 0 and got[1].tolist() == [28, 29, 30, 31, 36, 37, 38]
