@@ -726,7 +726,6 @@ POCKET_TTS_API int ptts_paged_plan(const PttsPagedPlan* plan, int device, void* 
         ptts::check_paged_plan(*plan);
         OnDevice on(device);
         ptts::launch_paged_plan(*plan, static_cast<hipStream_t>(stream));
-        ptts::check_launches("the block-table plan");
         return 0;
     });
 }
@@ -745,7 +744,6 @@ POCKET_TTS_API int ptts_rotary_append(const PttsRotaryAppend* args, int device, 
         ptts::check_rotary_append(*args);
         OnDevice on(device);
         ptts::launch_rotary_append(*args, static_cast<hipStream_t>(stream));
-        ptts::check_launches("the rotary append");
         return 0;
     });
 }
@@ -768,7 +766,6 @@ POCKET_TTS_API int ptts_paged_attention(const PttsPagedAttention* args, int devi
         ptts::check_paged_attention(*args);
         OnDevice on(device);
         ptts::launch_paged_attention(*args, compute_units(device), static_cast<hipStream_t>(stream));
-        ptts::check_launches("the paged attention");
         return 0;
     });
 }

@@ -5,6 +5,9 @@
 
 #include <hip/hip_runtime.h>
 
+#include <stdexcept>
+#include <string>
+
 #include "pocket_tts/pocket_tts_amd.h"
 
 namespace ptts {
@@ -16,6 +19,17 @@ void launch_paged_plan(const PttsPagedPlan& p, hipStream_t s);
 void launch_rotary_append(const PttsRotaryAppend& a, hipStream_t s);
 long long paged_attention_workspace(const PttsPagedAttention& a, int cus);
 void launch_paged_attention(const PttsPagedAttention& a, int cus, hipStream_t s);
+
+// One launch, its own error thrown.  The thread's last error is not asked: it may come from any earlier call of the program (a poll of a
+// stream that is not ready sets it), and is left as it was.
+template <typename A> void launch_paged(void (*kernel)(A), dim3 grid, hipStream_t s, A a) {
+    void* args[] = {&a};
+    const hipError_t e = hipLaunchKernel(reinterpret_cast<const void*>(kernel), grid, dim3(256), args, 0, s);
+    if (e != hipSuccess) {
+        (void)hipGetLastError();          // this one has been reported
+        throw std::runtime_error(std::string("kernel launch failed: ") + hipGetErrorString(e));
+    }
+}
 
 // The part of the checks that two of them share.
 void check_pages(const PttsPages& p, const char* who);

@@ -877,8 +877,8 @@ Cut cut_of(const PttsPagedAttention& p, int cus) {
 }
 
 template <typename T, typename C, int DH> void launch_few_of(const AttnArgs& a, unsigned grid, hipStream_t s) {
-    if (a.p.pages.head_dim == DH) hipLaunchKernelGGL((attention_few_kernel<T, C, DH, true>), dim3(grid), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((attention_few_kernel<T, C, DH, false>), dim3(grid), dim3(256), 0, s, a);
+    if (a.p.pages.head_dim == DH) launch_paged(attention_few_kernel<T, C, DH, true>, dim3(grid), s, a);
+    else launch_paged(attention_few_kernel<T, C, DH, false>, dim3(grid), s, a);
 }
 template <typename T, typename C> void launch_few(const AttnArgs& a, unsigned grid, hipStream_t s) {
     const int d = a.p.pages.head_dim;
@@ -888,9 +888,9 @@ template <typename T, typename C> void launch_few(const AttnArgs& a, unsigned gr
 }
 template <typename T> void launch_chunk(const AttnArgs& a, unsigned grid, hipStream_t s) {
     const int d = a.p.pages.head_dim;
-    if (d <= 64) hipLaunchKernelGGL((attention_chunk_kernel<T, 64>), dim3(grid), dim3(256), 0, s, a);
-    else if (d <= 128) hipLaunchKernelGGL((attention_chunk_kernel<T, 128>), dim3(grid), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((attention_chunk_kernel<T, 256>), dim3(grid), dim3(256), 0, s, a);
+    if (d <= 64) launch_paged(attention_chunk_kernel<T, 64>, dim3(grid), s, a);
+    else if (d <= 128) launch_paged(attention_chunk_kernel<T, 128>, dim3(grid), s, a);
+    else launch_paged(attention_chunk_kernel<T, 256>, dim3(grid), s, a);
 }
 
 // A launch holds fewer than 2^32 threads.
@@ -966,9 +966,9 @@ void launch_paged_attention(const PttsPagedAttention& p, int cus, hipStream_t s)
     if (c.bytes > 0) {
         const long long items = static_cast<long long>(p.q_heads) * (p.pages.head_dim / 4);
         const dim3 merge(p.rows, static_cast<unsigned>((items + 255) / 256));
-        if (p.q_type == PTTS_TYPE_F32) hipLaunchKernelGGL(attention_merge_kernel<float>, merge, dim3(256), 0, s, a);
-        else if (p.q_type == PTTS_TYPE_BF16) hipLaunchKernelGGL(attention_merge_kernel<__bf16>, merge, dim3(256), 0, s, a);
-        else hipLaunchKernelGGL(attention_merge_kernel<_Float16>, merge, dim3(256), 0, s, a);
+        if (p.q_type == PTTS_TYPE_F32) launch_paged(attention_merge_kernel<float>, merge, s, a);
+        else if (p.q_type == PTTS_TYPE_BF16) launch_paged(attention_merge_kernel<__bf16>, merge, s, a);
+        else launch_paged(attention_merge_kernel<_Float16>, merge, s, a);
     }
 }
 

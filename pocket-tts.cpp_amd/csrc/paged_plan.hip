@@ -197,8 +197,8 @@ void launch_paged_plan(const PttsPagedPlan& p, hipStream_t s) {
     a.picks = most < p.n_free ? most : p.n_free;
     const long long slices = std::max<long long>((p.rows + kSlice - 1) / kSlice, (a.picks + kSlice - 1) / kSlice);
     const dim3 grid(static_cast<unsigned>(std::max<long long>(slices, 1)));
-    if (p.requests <= 256) hipLaunchKernelGGL(plan_kernel<1>, grid, dim3(256), 0, s, a);
-    else hipLaunchKernelGGL(plan_kernel<4>, grid, dim3(256), 0, s, a);
+    if (p.requests <= 256) launch_paged(plan_kernel<1>, grid, s, a);
+    else launch_paged(plan_kernel<4>, grid, s, a);
 }
 
 }  // namespace ptts

@@ -150,20 +150,20 @@ void dispatch(RotaryArgs a, bool wide, hipStream_t s) {
     a.per_v = FastDiv::of(static_cast<unsigned>(per_v));
     a.units = rot_heads * per_head + (p.k ? p.pages.kv_heads * per_v : 0);
     // One row a workgroup (two took 37.9 us in place of 34.6 for the 8192 rows below), and up to four workgroups a row where rows are few.
-    const dim3 grid(p.rows, std::min(4, std::max(1, 256 / p.rows))), block(256);
+    const dim3 grid(p.rows, std::min(4, std::max(1, 256 / p.rows)));
     // What is more than the L2 caches hold between them (8 x 4 MB) cannot wait there for its reader, and passing it through them costs:
     // 8192 rows of 48 heads of 128 in bf16 (201 MB) take 41.9 us through the caches and 34.6 us past them (5.8 TB/s).  Smaller calls stay in
     // the caches, where the attention that follows finds them.
     const long long moved = static_cast<long long>(p.rows) * p.pages.head_dim * ((p.q ? 2ll * p.q_heads * sizeof(T) : 0) + (p.k ? 2ll * p.pages.kv_heads * (sizeof(T) + sizeof(C)) : 0));
     const bool stream = moved > 32ll << 20;
     if (wide) {
-        if (p.interleaved && stream) hipLaunchKernelGGL((rotary_kernel<T, C, W, true, true>), grid, block, 0, s, a);
-        else if (p.interleaved) hipLaunchKernelGGL((rotary_kernel<T, C, W, true, false>), grid, block, 0, s, a);
-        else if (stream) hipLaunchKernelGGL((rotary_kernel<T, C, W, false, true>), grid, block, 0, s, a);
-        else hipLaunchKernelGGL((rotary_kernel<T, C, W, false, false>), grid, block, 0, s, a);
+        if (p.interleaved && stream) launch_paged(rotary_kernel<T, C, W, true, true>, grid, s, a);
+        else if (p.interleaved) launch_paged(rotary_kernel<T, C, W, true, false>, grid, s, a);
+        else if (stream) launch_paged(rotary_kernel<T, C, W, false, true>, grid, s, a);
+        else launch_paged(rotary_kernel<T, C, W, false, false>, grid, s, a);
     } else {
-        if (p.interleaved) hipLaunchKernelGGL((rotary_kernel<T, C, 1, true, false>), grid, block, 0, s, a);
-        else hipLaunchKernelGGL((rotary_kernel<T, C, 1, false, false>), grid, block, 0, s, a);
+        if (p.interleaved) launch_paged(rotary_kernel<T, C, 1, true, false>, grid, s, a);
+        else launch_paged(rotary_kernel<T, C, 1, false, false>, grid, s, a);
     }
 }
 

@@ -35,3 +35,21 @@ def test_plan_reports_free_pages_that_are_none():
     assert status == 1 and got[1].tolist() == [28, 29, 30, 31, -1, 36, 37, 38]
     got, status = _run_plan([0, 0], [4, 3], 4, np.full((2, 3), -1), np.array([7, 9, -1]), 7)
     assert status == 0 and got[1].tolist() == [28, 29, 30, 31, 36, 37, 38]
+
+
+def test_an_error_from_before_the_call_is_not_the_calls():
+    """The thread's last error belongs to whoever made it: a call that launches reports its own launches alone and leaves it."""
+    import ctypes as C
+
+    from test_paged_gpu_use import Loop, _clear_slots, _hip
+    h = _hip()
+    h.hipSetDevice.argtypes, h.hipGetLastError.argtypes = [C.c_int], []
+    loop, rng = Loop(), np.random.default_rng(0)
+    for arriving in ((3, 1, 20), (1, 1, 1)):
+        loop.feed(arriving, rng)
+        _clear_slots(loop)
+        bad = h.hipSetDevice(99)
+        assert bad != 0
+        loop.launch()
+        assert h.hipGetLastError() == bad
+        loop.check()
