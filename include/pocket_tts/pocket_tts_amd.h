@@ -160,7 +160,7 @@ POCKET_TTS_API int ptts_mimi_encode_batch(PocketTTSHandle handle, const float* c
  * Unlike the calls above, these take DEVICE pointers of GPU `device`, enqueue on `stream` (a hipStream_t; NULL: the device's
  * default stream) and return without waiting: 0, or -1 with a message and nothing launched.  They allocate nothing, keep nothing
  * between calls, may be called from several threads at once and may be captured into a graph.  Buffers must not overlap unless
- * stated.  Strides count elements; the last axis is contiguous.  Values in device memory (lengths, page ids, slots) are checked
+ * stated.  Addresses are multiples of their type's size.  Strides count elements; the last axis is contiguous.  Values in device memory (lengths, page ids, slots) are checked
  * by the kernels: what is out of range is not read or written and sets a bit of *status (may be NULL; the caller clears it):
  * 1 page id or slot outside the pool, 2 row ranges outside the rows or not ascending, 4 a length negative or beyond its table. */
 enum { PTTS_TYPE_F32 = 0, PTTS_TYPE_BF16 = 1, PTTS_TYPE_F16 = 2 };

@@ -5,6 +5,8 @@
 
 #include <hip/hip_runtime.h>
 
+#include <cstdint>
+#include <initializer_list>
 #include <stdexcept>
 #include <string>
 
@@ -35,6 +37,13 @@ template <typename A> void launch_paged(void (*kernel)(A), dim3 grid, hipStream_
 void check_pages(const PttsPages& p, const char* who);
 
 constexpr int kStatusPage = 1, kStatusRows = 2, kStatusLength = 4;
+
+// Whether all of these addresses (null ones too) are multiples of n.
+inline bool aligned(std::initializer_list<const void*> ptrs, unsigned n) {
+    uintptr_t low = 0;
+    for (const void* p : ptrs) low |= reinterpret_cast<uintptr_t>(p);
+    return low % n == 0;
+}
 
 inline int type_size(int t) { return t == PTTS_TYPE_F32 ? 4 : 2; }
 

@@ -921,6 +921,8 @@ void check_paged_attention(const PttsPagedAttention& p) {
     if (p.rows == 0 || p.requests == 0) return;
     if (!p.q || !p.out || !p.cu_rows || !p.kv_len || (p.table_width > 0 && !p.block_table))
         throw std::runtime_error(w + "q, out, cu_rows, kv_len and block_table are required");
+    if (!aligned({p.block_table, p.cu_rows, p.kv_len, p.lse, p.status}, 4))
+        throw std::runtime_error(w + "block_table, cu_rows, kv_len, lse and status must be aligned to 4 bytes");
     if (p.q == p.out) throw std::runtime_error(w + "out must not be q");
     const int e = 16 / type_size(p.q_type);
     if (reinterpret_cast<uintptr_t>(p.q) % 16 || p.q_row_stride % e || p.q_head_stride % e || reinterpret_cast<uintptr_t>(p.out) % 16 ||

@@ -185,6 +185,8 @@ void check_paged_plan(const PttsPagedPlan& p) {
         throw std::runtime_error("cached, arriving, kv_len and block_table are required");
     if (!p.cu_rows || !p.counts) throw std::runtime_error("cu_rows and counts are required");
     if (p.rows > 0 && (!p.slot_map || !p.positions)) throw std::runtime_error("slot_map and positions are required");
+    if (!aligned({p.cached, p.arriving, p.free_pages, p.block_table, p.slot_map, p.positions, p.cu_rows, p.kv_len, p.counts, p.status}, 4))
+        throw std::runtime_error("all arrays must be aligned to 4 bytes");
     if (p.n_free > 0 && !p.free_pages) throw std::runtime_error("free_pages is required");
 }
 

@@ -213,6 +213,8 @@ void check_rotary_append(const PttsRotaryAppend& p) {
     if (p.k && !p.slot_map) throw std::runtime_error(w + "slot_map is required");
     if (p.q == p.q_out && p.q && (p.q_row_stride != p.out_row_stride || p.q_head_stride != p.out_head_stride))
         throw std::runtime_error(w + "q_out may be q itself only with the same strides");
+    if (!aligned({p.positions, p.slot_map, p.status}, 4) || !aligned({p.freq}, 8))
+        throw std::runtime_error(w + "positions, slot_map and status must be aligned to 4 bytes, freq to 8");
     if (low_bits(p) % type_size(p.type)) throw std::runtime_error(w + "rows must be aligned to their type");
 }
 

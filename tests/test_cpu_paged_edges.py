@@ -41,3 +41,30 @@ def test_workspace_query_with_an_explicit_none():
     passes_checks(ptts_paged.attention_workspace, *lead, out=None)
     with pytest.raises(ptts_lib.PttsError, match="must not be q"):
         ptts_paged.attention_workspace(*lead, out=x)
+
+
+@pytest.mark.parametrize("name,dtype", [("cached", "int32"), ("free_pages", "int32"), ("block_table", "int32"), ("counts", "int32"), ("status", "int32")])
+def test_plan_refuses_what_is_not_aligned(name, dtype):
+    """Arrays off their type's alignment: an atomic on such an address faults."""
+    shapes = dict(cached=(3,), arriving=(3,), free_pages=(9,), block_table=(3, 5), slot_map=(7,), positions=(7,), cu_rows=(4,), kv_len=(3,), counts=(4,), status=(1,))
+    a = {k: arr(s, ptr=PTR + 2 * (k == name)) for k, s in shapes.items()}
+    with pytest.raises(ptts_lib.PttsError, match="aligned"):
+        ptts_paged.plan(a.pop("cached"), a.pop("arriving"), a.pop("free_pages"), a.pop("block_table"), 16, **a)
+
+
+@pytest.mark.parametrize("name", ["positions", "slot_map", "freq", "status"])
+def test_rotary_refuses_what_is_not_aligned(name):
+    x, kv, pages = arr((5, 4, 64), "bfloat16"), arr((5, 2, 64), "bfloat16"), arr((9, 16, 2, 64), "bfloat16")
+    a = {k: arr(s, t, ptr=PTR + (4 if t == "float64" else 2) * (k == name)) for k, s, t in (("positions", (5,), "int32"), ("slot_map", (5,), "int32"),
+                                                                                       ("freq", (32,), "float64"), ("status", (1,), "int32"))}
+    with pytest.raises(ptts_lib.PttsError, match="aligned"):
+        ptts_paged.rotary_append(x, kv, kv, a.pop("positions"), a.pop("freq"), k_pages=pages, v_pages=pages, **a)
+
+
+@pytest.mark.parametrize("name", ["block_table", "cu_rows", "kv_len", "lse", "status"])
+def test_attention_refuses_what_is_not_aligned(name):
+    x, out, pages = arr((5, 4, 64), "bfloat16"), arr((5, 4, 64), "bfloat16", ptr=2 * PTR), arr((9, 16, 2, 64), "bfloat16")
+    a = {k: arr(s, t, ptr=PTR + 2 * (k == name)) for k, s, t in (("block_table", (3, 5), "int32"), ("cu_rows", (4,), "int32"), ("kv_len", (3,), "int32"),
+                                                                 ("lse", (5, 4), "float32"), ("status", (1,), "int32"))}
+    with pytest.raises(ptts_lib.PttsError, match="aligned"):
+        ptts_paged.attention(x, pages, pages, a.pop("block_table"), a.pop("cu_rows"), a.pop("kv_len"), out=out, **a)
