@@ -51,7 +51,7 @@ struct AttnArgs {
     PttsPagedAttention p;
     FastDiv page, group;
     float scale2;               // scale * log2(e)
-    long long tiles;
+    long long tile0, tile1;     // tiles of this launch: tile0 .. tile1 - 1
     int splits, least;
     // results of splits: [split][row][head][dim] values, normalised by the split's own sum, and [split][row][head] of log2 sum exp2
     float *part, *lse;
@@ -249,7 +249,7 @@ template <typename T, int DH> __global__ __launch_bounds__(256, DH == 256 ? 1 : 
     const unsigned rest = block / p.pages.kv_heads;
     const int splits = a.splits, split = rest % splits;
     Tile t;
-    if (!find_tile(a, a.tiles - 1 - rest / splits, kChunkRows, t)) return;
+    if (!find_tile(a, a.tile1 - 1 - rest / splits, kChunkRows, t)) return;
     const int G = a.group.d, dim = p.pages.head_dim;
     const Blocks list(t, p.sinks, kChunkKeys);
     const int per = max(a.least, (list.count + splits - 1) / splits);
@@ -513,7 +513,7 @@ __global__ __launch_bounds__(256, DH == 256 ? 1 : DH == 128 ? 2 : 3) void attent
     const unsigned rest = block / p.pages.kv_heads;
     const int splits = a.splits, split = rest % splits;
     Tile t;
-    if (!find_tile(a, rest / splits, kFewRows, t)) return;
+    if (!find_tile(a, a.tile0 + rest / splits, kFewRows, t)) return;
     const int G = a.group.d, dim = p.pages.head_dim;
     const Blocks list(t, p.sinks, kKeys);
     const int per = max(a.least, (list.count + splits - 1) / splits);
@@ -894,10 +894,7 @@ template <typename T> void launch_chunk(const AttnArgs& a, unsigned grid, hipStr
 }
 
 // A launch holds fewer than 2^32 threads.
-unsigned grid_of(long long n) {
-    if (n >= 1 << 24) throw std::runtime_error("paged_attention: too many rows and heads for one call");
-    return static_cast<unsigned>(n);
-}
+constexpr long long kMostGroups = (1 << 24) - 1;
 
 }  // namespace
 
@@ -940,30 +937,34 @@ void launch_paged_attention(const PttsPagedAttention& p, int cus, hipStream_t s)
             throw std::runtime_error("paged_attention: a workspace of " + std::to_string(c.bytes) + " bytes is required");
         if (reinterpret_cast<uintptr_t>(p.workspace) % 16) throw std::runtime_error("paged_attention: the workspace must be aligned to 16 bytes");
     }
-    const unsigned grid = grid_of(c.tiles * c.splits * p.pages.kv_heads);
     AttnArgs a;
     a.p = p;
     if (p.window > 1 << 30) a.p.window = 0;          // no context is that long
     a.page = FastDiv::of(static_cast<unsigned>(p.pages.page_size));
     a.group = FastDiv::of(static_cast<unsigned>(p.q_heads / p.pages.kv_heads));
     a.scale2 = p.scale * 1.4426950408889634f;
-    a.tiles = c.tiles;
     a.splits = c.splits;
     a.least = c.least;
     a.part = static_cast<float*>(p.workspace);
     a.lse = a.part + c.splits * c.parts * p.pages.head_dim;
     a.parts = c.parts;
-    if (c.chunk) {
-        if (p.q_type == PTTS_TYPE_BF16) launch_chunk<__bf16>(a, grid, s);
-        else launch_chunk<_Float16>(a, grid, s);
-    } else if (p.q_type == PTTS_TYPE_F32 && p.pages.type == PTTS_TYPE_BF16) {
-        launch_few<float, __bf16>(a, grid, s);
-    } else if (p.q_type == PTTS_TYPE_F32) {
-        launch_few<float, float>(a, grid, s);
-    } else if (p.q_type == PTTS_TYPE_BF16) {
-        launch_few<__bf16, __bf16>(a, grid, s);
-    } else {
-        launch_few<_Float16, _Float16>(a, grid, s);
+    // all tiles in one launch, as far as one holds them
+    const long long groups = static_cast<long long>(c.splits) * p.pages.kv_heads, most = kMostGroups / groups;
+    for (a.tile0 = 0; a.tile0 < c.tiles; a.tile0 = a.tile1) {
+        a.tile1 = std::min(a.tile0 + most, c.tiles);
+        const unsigned grid = static_cast<unsigned>((a.tile1 - a.tile0) * groups);
+        if (c.chunk) {
+            if (p.q_type == PTTS_TYPE_BF16) launch_chunk<__bf16>(a, grid, s);
+            else launch_chunk<_Float16>(a, grid, s);
+        } else if (p.q_type == PTTS_TYPE_F32 && p.pages.type == PTTS_TYPE_BF16) {
+            launch_few<float, __bf16>(a, grid, s);
+        } else if (p.q_type == PTTS_TYPE_F32) {
+            launch_few<float, float>(a, grid, s);
+        } else if (p.q_type == PTTS_TYPE_BF16) {
+            launch_few<__bf16, __bf16>(a, grid, s);
+        } else {
+            launch_few<_Float16, _Float16>(a, grid, s);
+        }
     }
     if (c.bytes > 0) {
         const long long items = static_cast<long long>(p.q_heads) * (p.pages.head_dim / 4);

@@ -37,6 +37,26 @@ def test_plan_reports_free_pages_that_are_none():
     assert status == 0 and got[1].tolist() == [28, 29, 30, 31, 36, 37, 38]
 
 
+def test_a_step_without_rows():
+    """Nothing arrives: all three calls run and leave everything as it was."""
+    import ptts_paged
+    from ptts_paged import DeviceArray
+    d = {k: ref.Dev(np.asarray(v), "int32") for k, v in dict(cached=[5, 0], arriving=[0, 0], free=[3], table=[[1, -1], [-1, -1]], cu=[9, 9, 9], kv_len=[9, 9],
+                                                             counts=np.full(4, 9), status=[0]).items()}
+    none = lambda dtype, *shape: DeviceArray(0, shape, dtype)
+    ptts_paged.plan(d["cached"].a, d["arriving"].a, d["free"].a, d["table"].a, 4, slot_map=none("int32", 0), positions=none("int32", 0), cu_rows=d["cu"].a,
+                    kv_len=d["kv_len"].a, counts=d["counts"].a, status=d["status"].a)
+    assert d["cu"].host().tolist() == [0, 0, 0] and d["kv_len"].host().tolist() == [5, 0] and d["counts"].host().tolist() == [0, 0, 0, 0]
+    assert d["table"].host().tolist() == [[1, -1], [-1, -1]]
+    k0 = np.random.default_rng(0).standard_normal((4, 4, 2, 64)).astype(np.float32)
+    pages, freq = ref.floats(k0, "float32"), ref.Dev(np.ones(32), "float64")
+    q, k = none("float32", 0, 4, 64), none("float32", 0, 2, 64)
+    ptts_paged.rotary_append(q, k, k, none("int32", 0), freq.a, slot_map=none("int32", 0), k_pages=pages.a, v_pages=pages.a, status=d["status"].a)
+    ptts_paged.attention(q, pages.a, pages.a, d["table"].a, d["cu"].a, d["kv_len"].a, out=q, lse=none("float32", 0, 4), status=d["status"].a)
+    np.testing.assert_array_equal(pages.host(), k0)
+    assert d["status"].host()[0] == 0
+
+
 def test_an_error_from_before_the_call_is_not_the_calls():
     """The thread's last error belongs to whoever made it: a call that launches reports its own launches alone and leaves it."""
     import ctypes as C
@@ -53,3 +73,26 @@ def test_an_error_from_before_the_call_is_not_the_calls():
         loop.launch()
         assert h.hipGetLastError() == bad
         loop.check()
+
+
+@pytest.mark.parametrize("kind", ["float16", "float32"])
+def test_attention_beyond_one_launch(kind):
+    """More workgroups than one launch holds (2^24): 65536 requests of one row and one key, 256 heads of 8."""
+    import ptts_paged
+    n, heads, dim, pages = 65536, 256, 8, 64
+    rng = np.random.default_rng(1)
+    v = ref.rounded(rng.standard_normal((pages, 1, heads, dim)), kind)
+    page_of = rng.integers(0, pages, n)
+    page_of[:2] = 0, 1
+    row = rng.standard_normal((heads, dim))
+    d = [ref.floats(np.broadcast_to(row, (n, heads, dim)), kind), ref.floats(rng.standard_normal((pages, 1, heads, dim)), kind), ref.floats(v, kind),
+         ref.floats(np.zeros((n, heads, dim)), kind)]
+    ints = [ref.Dev(x, "int32") for x in (page_of[:, None], np.arange(n + 1), np.ones(n), np.zeros(1))]
+    a = [x.a for x in d[:3]] + [x.a for x in ints[:3]]
+    assert ptts_paged.attention_workspace(*a, out=d[3].a, max_rows=1, max_kv=1) == 0
+    ptts_paged.attention(*a, out=d[3].a, status=ints[3].a, max_rows=1, max_kv=1)
+    # One key: its value.  The kernel forms v w / w with a weight w near 1: a product, a reciprocal and a product in float32, each off by at most
+    # 2^-24 of its result, so 3.01 2^-24 in all.  Half a step of float16 is 2^-11: there it rounds back to v.
+    off = np.abs(ref.from_bits(d[3].host(), kind) - v[page_of, 0])
+    assert (off <= (3.01 * 2.0 ** -24 * np.abs(v[page_of, 0]) if kind == "float32" else 0.0)).all(), off.max()
+    assert ints[3].host()[0] == 0
