@@ -109,7 +109,8 @@ POCKET_TTS_API int ptts_state_reset(PocketTTSHandle handle, void* state);
  * in chunks); a call that needs more pages than are free fails and changes nothing.  No counterpart in the reference. */
 POCKET_TTS_API void* ptts_state_new_paged(PocketTTSHandle handle, int batch, int pages, int page_size, int max_context, int window, int sinks);
 /* Slot to_slot of a paged state begins anew with the first `rows` rows of from_slot (one voice for many utterances): whole pages
- * are shared, the rest is copied. */
+ * are shared, the rest is copied.  The slot's own pages go back to the pool (and serve for the copy); rows that from_slot has given back
+ * cannot be shared.  The LM's state alone: the codec's state of to_slot stays as it is. */
 POCKET_TTS_API int ptts_state_share(PocketTTSHandle handle, void* state, int from_slot, int to_slot, int rows);
 /* Free pages of a paged state's pool. */
 POCKET_TTS_API int ptts_state_free_pages(PocketTTSHandle handle, void* state);
@@ -233,8 +234,12 @@ POCKET_TTS_API int ptts_rotary_append(const PttsRotaryAppend* args, int device, 
  * kv_len[i] - 1 for the last of them (so their own keys are in the pages already).  The query at position p sees key j if j <= p and
  * (window <= 0 or j > p - window or j < sinks).  out = softmax(scale q.k) v, lse (may be NULL) = ln sum exp(scale q.k); a row that
  * sees nothing gets 0 and -inf.  Head h of q reads head h / (q_heads / kv_heads) of the pages.  Keys that a row does not see
- * never reach it, whatever they hold.  out may not alias q.
- * rows * (q_heads / kv_heads) < 2^30.  Types: q and out q_type; pages of q_type, or bf16 pages under f32 rows.  Rows outside every request stay as they were.
+ * never reach it, whatever they hold.  A key that a row sees and whose page id is not one of the pool's (-1 of a plan that ran out of
+ * pages too) counts as a row of zeros, in k and in v, and sets status 1: check the plan's counts or the status.  out may not alias q.
+ * rows * (q_heads / kv_heads) < 2^30.  Types: q and out q_type; pages of q_type, or bf16 pages under f32 rows.  q and out and their strides
+ * are multiples of 16 bytes.  Rows outside every request stay as they were.
+ * Rounding: scores, softmax statistics and sums are float32; bf16 and f16 rows round each weight to their type before it meets its value
+ * (half a step on each weight, beside the result's own half step), f32 rows keep float32 weights.
  * max_rows, max_kv: what the caller knows of the largest row count and length of a request (0: nothing).  They choose how the work
  * is cut and cost time when wrong, never results.
  * workspace: ptts_paged_attention_workspace() bytes (0: none needed; -1: bad arguments), 16-byte aligned, contents irrelevant
