@@ -68,3 +68,15 @@ def test_attention_refuses_what_is_not_aligned(name):
                                                                  ("lse", (5, 4), "float32"), ("status", (1,), "int32"))}
     with pytest.raises(ptts_lib.PttsError, match="aligned"):
         ptts_paged.attention(x, pages, pages, a.pop("block_table"), a.pop("cu_rows"), a.pop("kv_len"), out=out, **a)
+
+
+def test_make_without_python_headers():
+    """The library and the programs are made where Python's headers are missing; with them the binding is made, too."""
+    import os
+    import subprocess
+    for inc, there in (("/nowhere", False), (None, True)):
+        cmd = ["make", "-n", "-C", ptts_lib.PKG, "all", f"OBJDIR={ptts_lib.PKG}/no_such_build"] + ([f"PYINC={inc}"] if inc else [])
+        r = subprocess.run(cmd + ["-W", os.path.join(ptts_lib.PKG, "csrc", "py_paged.cpp")], capture_output=True, text=True)
+        assert r.returncode == 0, r.stderr
+        assert ("py_paged.cpp" in r.stdout) == there and "c_api.cpp" in r.stdout
+        assert ("no Python headers" in r.stdout) != there
