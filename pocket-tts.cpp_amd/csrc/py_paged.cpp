@@ -37,6 +37,8 @@ constexpr int kCuda = 2, kRocm = 10;
 PyObject *g_error = nullptr;       // ptts_lib.PttsError
 PyObject *g_bind = nullptr;        // callable(with_torch): loads the library and calls bind()
 PyObject *g_allocate = nullptr;    // callable(device, bytes, stream or None): a torch tensor for the workspace
+PyObject *g_records = nullptr;     // callable(): whether torch records gradients now
+PyObject *g_needs_grad = nullptr;  // "requires_grad"
 int g_runtime = 0;                 // 0: not bound, 1: the system's runtime, 2: torch's
 
 struct Entries {
@@ -100,6 +102,24 @@ const DlApi* api_of(PyTypeObject* type) {
     return api;
 }
 
+// A tensor that requires gradients is refused while torch records them: these calls would drop them without a word.
+bool no_gradient(PyObject* o, const char* name) {
+    PyObject* needs = PyObject_GetAttr(o, g_needs_grad);
+    if (!needs) {
+        PyErr_Clear();
+        return true;
+    }
+    const bool maybe = needs != Py_False;
+    Py_DECREF(needs);
+    if (!maybe) return true;
+    PyObject* records = PyObject_CallNoArgs(g_records);
+    if (!records) return false;
+    const int on = PyObject_IsTrue(records);
+    Py_DECREF(records);
+    if (on < 0) return false;
+    return !on || fail("%s: requires gradients, which these calls do not record: detach it, or call under torch.no_grad()%s", name);
+}
+
 // Any array; false with an exception set.
 bool read(PyObject* o, const char* name, View& v) {
     v.name = name;
@@ -115,6 +135,7 @@ bool read(PyObject* o, const char* name, View& v) {
     } else {
         v.api = api_of(Py_TYPE(o));
         if (!v.api) return fail("%s: a torch tensor on the GPU or a DeviceArray is required, got %s", name, Py_TYPE(o)->tp_name);
+        if (!no_gradient(o, name)) return false;
         DlTensor t;
         if (v.api->view(o, &t) != 0) return false;
         if (t.device.type != kCuda && t.device.type != kRocm) return fail("%s: the tensor is not on the GPU%s", name);
@@ -570,10 +591,10 @@ PyObject* frequencies(PyObject*, PyObject* args) {
 }
 
 PyObject* setup(PyObject*, PyObject* args) {
-    PyObject *error, *bind, *allocate;
-    if (!PyArg_ParseTuple(args, "OOO", &error, &bind, &allocate)) return nullptr;
-    Py_INCREF(error); Py_INCREF(bind); Py_INCREF(allocate);
-    g_error = error; g_bind = bind; g_allocate = allocate;
+    PyObject *error, *bind, *allocate, *records;
+    if (!PyArg_ParseTuple(args, "OOOO", &error, &bind, &allocate, &records)) return nullptr;
+    Py_INCREF(error); Py_INCREF(bind); Py_INCREF(allocate); Py_INCREF(records);
+    g_error = error; g_bind = bind; g_allocate = allocate; g_records = records;
     Py_RETURN_NONE;
 }
 
@@ -623,6 +644,7 @@ PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_ptts_paged", "C side of ptts_pa
 PyMODINIT_FUNC PyInit__ptts_paged(void) {
     for (Names* n : {&g_plan_names, &g_rotary_names, &g_workspace_names, &g_attention_names})
         if (!intern(*n)) return nullptr;
+    if (!(g_needs_grad = PyUnicode_InternFromString("requires_grad"))) return nullptr;
     PyObject* type = PyType_FromSpec(&g_device_array_spec);
     if (!type) return nullptr;
     g_device_array = reinterpret_cast<PyTypeObject*>(type);

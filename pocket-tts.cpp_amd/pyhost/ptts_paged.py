@@ -7,7 +7,7 @@ library (the first call here does it too).
 
 Every call enqueues on `stream` (a torch stream or a handle; default: torch's current stream of the tensors' device, the default
 stream for DeviceArray) and returns without waiting.  Nothing is kept between calls.  Failures raise ptts_lib.PttsError.
-For inference: nothing is recorded for torch's autograd.
+For inference: nothing is recorded for torch's autograd, and a tensor that requires gradients is refused while torch records them.
 """
 from __future__ import annotations
 
@@ -49,7 +49,12 @@ def _allocate(device: int, size: int, stream):
         return torch.empty(size, dtype=torch.uint8, device=where)
 
 
-_c.setup(PttsError, _bind, _allocate)
+def _records_gradients() -> bool:
+    import torch
+    return torch.is_grad_enabled()
+
+
+_c.setup(PttsError, _bind, _allocate, _records_gradients)
 
 
 def frequencies(rot_dim: int, base: float = 10000.0, scaling: str = "none", factor: float = 1.0, trained: float = 0.0, fast: float = 32.0,
