@@ -134,6 +134,8 @@ bool read(PyObject* o, const char* name, View& v) {
         std::memcpy(v.strides, d->strides, sizeof v.strides);
     } else {
         v.api = api_of(Py_TYPE(o));
+        if (!v.api && PyObject_HasAttrString(o, "data_ptr"))
+            return fail("%s: %s publishes no exchange table (__dlpack_c_exchange_api__, in PyTorch from 2.10 on): pass a DeviceArray", name, Py_TYPE(o)->tp_name);
         if (!v.api) return fail("%s: a torch tensor on the GPU or a DeviceArray is required, got %s", name, Py_TYPE(o)->tp_name);
         if (!no_gradient(o, name)) return false;
         DlTensor t;

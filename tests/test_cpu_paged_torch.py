@@ -37,3 +37,26 @@ assert "not on the GPU" in said(lambda: P.rotary_append(x, None, None, pos, freq
 
 def test_tensors_that_require_gradients_are_refused():
     _run(GRAD)
+
+
+OLD = r'''
+class Tensor:                        # what a torch without the table looks like from here
+    def data_ptr(self):
+        return 0
+try:
+    P.rotary_append(Tensor(), None, None, None, None)
+except ptts_lib.PttsError as e:
+    assert "Tensor publishes no exchange table" in str(e), e
+else:
+    raise AssertionError("not refused")
+try:
+    P.rotary_append([1.0], None, None, None, None)
+except ptts_lib.PttsError as e:
+    assert "a torch tensor on the GPU or a DeviceArray is required, got list" in str(e), e
+else:
+    raise AssertionError("not refused")
+'''
+
+
+def test_tensors_without_the_exchange_table_are_told_so():
+    _run(OLD)
