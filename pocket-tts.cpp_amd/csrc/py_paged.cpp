@@ -137,9 +137,9 @@ bool read(PyObject* o, const char* name, View& v) {
         if (!v.api && PyObject_HasAttrString(o, "data_ptr"))
             return fail("%s: %s publishes no exchange table (__dlpack_c_exchange_api__, in PyTorch from 2.10 on): pass a DeviceArray", name, Py_TYPE(o)->tp_name);
         if (!v.api) return fail("%s: a torch tensor on the GPU or a DeviceArray is required, got %s", name, Py_TYPE(o)->tp_name);
-        if (!no_gradient(o, name)) return false;
         DlTensor t;
         if (v.api->view(o, &t) != 0) return false;
+        if (t.dtype.code != 0 && !no_gradient(o, name)) return false;         // integers have none
         if (t.device.type != kCuda && t.device.type != kRocm) return fail("%s: the tensor is not on the GPU%s", name);
         if (t.ndim > 8) return fail("%s: too many axes%s", name);
         v.ptr = static_cast<char*>(t.data) + t.byte_offset;
