@@ -1208,9 +1208,11 @@ __global__ __launch_bounds__(256, 4) void attn_decode_kernel(AttnDecodeArgs a) {
         }
     }
     if (!done) {
-        float4 q[16];
+        float4 q[KV16 ? 16 : 1];
+        if constexpr (KV16) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) q[i] = *(const float4*)(qs + 4 * i);
+            for (int i = 0; i < 16; ++i) q[i] = *(const float4*)(qs + 4 * i);
+        }
         for (int j = lane; j < cnt; j += 64) {
             const long long kr_ = cbase + (long long)((j0 + kb + j) % a.cap) * a.d;
             float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
