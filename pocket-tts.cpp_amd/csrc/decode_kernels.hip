@@ -31,6 +31,7 @@ namespace ptts {
 
 typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
 typedef __attribute__((ext_vector_type(4))) float f32x4;
+typedef __attribute__((ext_vector_type(4))) unsigned u32x4;
 
 template <typename CT> struct SkinnyTraits { static constexpr int kstep = 16, per = 4, kch = 128, pad = 4; };
 template <> struct SkinnyTraits<__bf16> { static constexpr int kstep = 32, per = 8, kch = 128, pad = 8; };
@@ -82,26 +83,29 @@ __global__ __launch_bounds__(256) void skinny_gemm_kernel(SkinnyArgs a) {
     const int k_begin = blockIdx.y * Kc;
     const int nchunks = (Kc + KCH - 1) / KCH;
     const int KS_total = a.K / KSTEP;
-    const uint4* wbase = (const uint4*)a.Wp + (long long)nt * KS_total * 64 + lane;
-    const uint4* wbase2 = (const uint4*)(W2 ? a.Wp2 : a.Wp) + (long long)nt * KS_total * 64 + lane;
+    // Every lane always loads: rows behind M and tiles behind N repeat the last ones (their results are not stored), and steps behind the
+    // slice's end read its start and are zeroed.  Loads under branches were merged with zeros, a move for each register and chunk.
+    const long long tile = min(nt, a.N / 16 - 1);
+    const u32x4* wbase = (const u32x4*)a.Wp + tile * KS_total * 64 + lane;
+    const u32x4* wbase2 = (const u32x4*)(W2 ? a.Wp2 : a.Wp) + tile * KS_total * 64 + lane;
 
-    float4 areg[APT];
-    uint4 bnext[NKS], bcur[NKS];
-    uint4 bnext2[W2 ? NKS : 1], bcur2[W2 ? NKS : 1];
-    auto load_chunk = [&](int c) {
+    f32x4 areg[APT];
+    u32x4 b0[NKS], b1[NKS], b0l[W2 ? NKS : 1], b1l[W2 ? NKS : 1];     // fragments of even and odd chunks, and their second terms
+    const float* arow[APT];
+#pragma unroll
+    for (int i = 0; i < APT; ++i) arow[i] = a.A + (long long)min(m0 + (tid + 256 * i) / PIECES, a.M - 1) * a.lda + k_begin;
+    auto load_chunk = [&](int c, u32x4 (&b)[NKS], u32x4 (&bl)[W2 ? NKS : 1]) {
         const int kc0 = c * KCH;  // offset inside the slice
 #pragma unroll
         for (int i = 0; i < APT; ++i) {
-            const int id = tid + 256 * i, row = id / PIECES, piece = id % PIECES;
-            const int k = kc0 + piece * 4;
-            const bool ok = (m0 + row) < a.M && k < Kc;
-            areg[i] = ok ? *(const float4*)(a.A + (long long)(m0 + row) * a.lda + k_begin + k) : make_float4(0.f, 0.f, 0.f, 0.f);
+            const int k = kc0 + (tid + 256 * i) % PIECES * 4;
+            areg[i] = *(const f32x4*)(arow[i] + (k < Kc ? k : 0));
         }
 #pragma unroll
         for (int i = 0; i < NKS; ++i) {
-            const int k = kc0 + i * KSTEP;
-            bnext[i] = (tile_live && k < Kc) ? wbase[(long long)((k_begin + k) / KSTEP) * 64] : make_uint4(0u, 0u, 0u, 0u);
-            if constexpr (W2) bnext2[i] = (tile_live && k < Kc) ? wbase2[(long long)((k_begin + k) / KSTEP) * 64] : make_uint4(0u, 0u, 0u, 0u);
+            const long long at = (long long)((k_begin + (kc0 + i * KSTEP < Kc ? kc0 + i * KSTEP : 0)) / KSTEP) * 64;
+            b[i] = wbase[at];
+            if constexpr (W2) bl[i] = wbase2[at];
         }
     };
 
@@ -113,53 +117,62 @@ __global__ __launch_bounds__(256) void skinny_gemm_kernel(SkinnyArgs a) {
     const float bias_col = (a.bias && !a.P && tile_live) ? a.bias[nt * 16 + r] : 0.f;
     const float cs_col = (a.colscale && !a.P && tile_live) ? a.colscale[nt * 16 + r] : 1.f;
 
-    load_chunk(0);
-    for (int c = 0; c < nchunks; ++c) {
+    auto chunk = [&](int c, u32x4 (&b)[NKS], u32x4 (&bl)[W2 ? NKS : 1], u32x4 (&next)[NKS], u32x4 (&nextl)[W2 ? NKS : 1]) {
         CT* buf = As[c & 1][0];
         CT* buf_lo = As[c & 1][PLANES - 1];
+        if ((c + 1) * KCH > Kc) {
+            const f32x4 zero_a = {0.f, 0.f, 0.f, 0.f};
+            const u32x4 zero_b = {0u, 0u, 0u, 0u};
+#pragma unroll
+            for (int i = 0; i < APT; ++i) areg[i] = c * KCH + (tid + 256 * i) % PIECES * 4 < Kc ? areg[i] : zero_a;
+#pragma unroll
+            for (int i = 0; i < NKS; ++i) {
+                b[i] = c * KCH + i * KSTEP < Kc ? b[i] : zero_b;
+                if constexpr (W2) bl[i] = c * KCH + i * KSTEP < Kc ? bl[i] : zero_b;
+            }
+        }
 #pragma unroll
         for (int i = 0; i < APT; ++i) {
             const int id = tid + 256 * i, row = id / PIECES, piece = id % PIECES;
             if constexpr (kBf16) {
                 bf16x4 hi, lo;
-                split_bf16(areg[i], hi, lo);
+                split_bf16(__builtin_bit_cast(float4, areg[i]), hi, lo);
                 *(bf16x4*)(buf + row * LDA + piece * 4) = hi;
                 *(bf16x4*)(buf_lo + row * LDA + piece * 4) = lo;
             } else {
-                *(float4*)(buf + row * LDA + piece * 4) = areg[i];
+                *(f32x4*)(buf + row * LDA + piece * 4) = areg[i];
             }
         }
-#pragma unroll
-        for (int i = 0; i < NKS; ++i) bcur[i] = bnext[i];
-        if constexpr (W2) {
-#pragma unroll
-            for (int i = 0; i < NKS; ++i) bcur2[i] = bnext2[i];
-        }
         __syncthreads();
-        if (c + 1 < nchunks) load_chunk(c + 1);
+        if (c + 1 < nchunks) load_chunk(c + 1, next, nextl);
 #pragma unroll
         for (int ks = 0; ks < NKS; ++ks) {
             if constexpr (!kBf16) {
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) {
                     const float4 a4 = *(const float4*)(buf + (mt * 16 + r) * LDA + ks * 16 + 4 * g);
-                    acc[mt] = __builtin_amdgcn_mfma_f32_16x16x4f32(a4.x, __uint_as_float(bcur[ks].x), acc[mt], 0, 0, 0);
-                    acc[mt] = __builtin_amdgcn_mfma_f32_16x16x4f32(a4.y, __uint_as_float(bcur[ks].y), acc[mt], 0, 0, 0);
-                    acc[mt] = __builtin_amdgcn_mfma_f32_16x16x4f32(a4.z, __uint_as_float(bcur[ks].z), acc[mt], 0, 0, 0);
-                    acc[mt] = __builtin_amdgcn_mfma_f32_16x16x4f32(a4.w, __uint_as_float(bcur[ks].w), acc[mt], 0, 0, 0);
+                    acc[mt] = __builtin_amdgcn_mfma_f32_16x16x4f32(a4.x, __uint_as_float(b[ks].x), acc[mt], 0, 0, 0);
+                    acc[mt] = __builtin_amdgcn_mfma_f32_16x16x4f32(a4.y, __uint_as_float(b[ks].y), acc[mt], 0, 0, 0);
+                    acc[mt] = __builtin_amdgcn_mfma_f32_16x16x4f32(a4.z, __uint_as_float(b[ks].z), acc[mt], 0, 0, 0);
+                    acc[mt] = __builtin_amdgcn_mfma_f32_16x16x4f32(a4.w, __uint_as_float(b[ks].w), acc[mt], 0, 0, 0);
                 }
             } else {
-                const bf16x8 b8 = __builtin_bit_cast(bf16x8, bcur[ks]);
+                const bf16x8 b8 = __builtin_bit_cast(bf16x8, b[ks]);
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) {
                     const bf16x8 lo8 = *(const bf16x8*)(buf_lo + (mt * 16 + r) * LDA + ks * 32 + 8 * g);
                     const bf16x8 hi8 = *(const bf16x8*)(buf + (mt * 16 + r) * LDA + ks * 32 + 8 * g);
-                    if constexpr (W2) acc[mt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hi8, __builtin_bit_cast(bf16x8, bcur2[ks]), acc[mt], 0, 0, 0);
+                    if constexpr (W2) acc[mt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hi8, __builtin_bit_cast(bf16x8, bl[ks]), acc[mt], 0, 0, 0);
                     acc[mt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(lo8, b8, acc[mt], 0, 0, 0);
                     acc[mt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hi8, b8, acc[mt], 0, 0, 0);
                 }
             }
         }
+    };
+    load_chunk(0, b0, b0l);
+    for (int c = 0; c < nchunks; c += 2) {
+        chunk(c, b0, b0l, b1, b1l);
+        if (c + 1 < nchunks) chunk(c + 1, b1, b1l, b0, b0l);
     }
     if (!tile_live) return;
     const int col = nt * 16 + r;
@@ -625,7 +638,6 @@ std::vector<unsigned char> pack_q8_layout(const signed char* q, int N, int K) {
 // weights and every row.  Products are accumulated in skinny_gemm_kernel's order (k-steps ascending, low term
 // before high term), so the result is the same bit for bit.
 constexpr int kWideK = 512, kWideKS = kWideK / 32, kWideAhead = 3, kWideLd = 64 + 8;
-typedef __attribute__((ext_vector_type(4))) unsigned u32x4;
 
 // MT: 16-row tiles per wave.  2: 32 rows per wave, 128 rows per workgroup.  1: 16 rows per wave, for row counts that fill
 // 64-row slabs only.  One workgroup per CU either way: two of the second form per CU (256 registers, a few spilled) were
@@ -1224,10 +1236,16 @@ __global__ __launch_bounds__(256, 4) void attn_decode_kernel(AttnDecodeArgs a) {
                     s0 += q[2 * i + 1].x * (float)k8[4]; s1 += q[2 * i + 1].y * (float)k8[5]; s2 += q[2 * i + 1].z * (float)k8[6]; s3 += q[2 * i + 1].w * (float)k8[7];
                 }
             } else {
+                // the whole key is asked for before any of it is used (left to itself the compiler keeps four pieces in flight); the
+                // query, which every lane reads alike, stays in LDS and leaves the registers to the key
+                float4 k4[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) k4[i] = *(const float4*)((const float*)a.kcache + kr_ + 4 * i);
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    const float4 k4 = *(const float4*)((const float*)a.kcache + kr_ + 4 * i);
-                    s0 += q[i].x * k4.x; s1 += q[i].y * k4.y; s2 += q[i].z * k4.z; s3 += q[i].w * k4.w;
+                    const float4 qi = *(const float4*)(qs + 4 * i);
+                    s0 += qi.x * k4[i].x; s1 += qi.y * k4[i].y; s2 += qi.z * k4[i].z; s3 += qi.w * k4[i].w;
                 }
             }
             const float sv = ((s0 + s1) + (s2 + s3)) * 0.125f;
