@@ -485,6 +485,9 @@ __global__ __launch_bounds__(kThreads) void flow_ring_kernel(FlowRingArgs a) {
                     p0[s] = ld_sc1(rs, p_off_prev + (unsigned)(s * BC * 4) + ro + c0 * 4);
                     p1[s] = ld_sc1(rs, p_off_prev + (unsigned)(s * BC * 4) + ro + c1 * 4);
                 }
+                // all slabs on their way before the first is used: left to itself the compiler put the first sum, and with it a wait for
+                // the four loads before it, in the middle of the loads
+                __builtin_amdgcn_sched_barrier(0);
                 float4 s0 = p0[0], s1 = p1[0];
 #pragma unroll
                 for (int s = 1; s < G; ++s) {
