@@ -183,7 +183,8 @@ typedef struct {
  * counts[4] = new rows in all (those beyond `rows` are not written), pages taken, pages missing, rows without a page.  A page that is missing (free list exhausted, or
  * table row full) leaves -1 in the table and its rows get slot -1, in later plans too.  An id below 0 in free_pages is entered as it
  * is and its rows get slot -1 (status 1; counts takes it for a page).  A negative length counts as 0.
- * Rows of slot_map and positions behind the last new row stay as they are.  The last page of a request must not be shared when
+ * Rows of slot_map and positions behind the last new row stay as they are: a loop that gives ptts_rotary_append more rows than arrive
+ * (a captured step of fixed size) sets its slot_map to -1 before the plan, or they name the slots of an earlier step.  The last page of a request must not be shared when
  * it is partly filled and rows arrive.  requests <= 65536. */
 typedef struct {
     const int* cached;

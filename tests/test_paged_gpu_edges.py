@@ -96,3 +96,21 @@ def test_attention_beyond_one_launch(kind):
     off = np.abs(ref.from_bits(d[3].host(), kind) - v[page_of, 0])
     assert (off <= (3.01 * 2.0 ** -24 * np.abs(v[page_of, 0]) if kind == "float32" else 0.0)).all(), off.max()
     assert ints[3].host()[0] == 0
+
+
+@pytest.mark.parametrize("hints", [(1, 1), (1, 1 << 30), (1 << 30, 1), (5, 64)])
+@pytest.mark.parametrize("kind", ["bfloat16", "float16", "float32"])
+def test_hints_that_are_wrong_change_no_results(kind, hints):
+    """max_rows and max_kv far from the truth: other forms and splits, the same results within the bounds."""
+    import ptts_paged
+    from test_paged_gpu import _attend, _compare
+    real, query = ptts_paged.attention, ptts_paged.attention_workspace
+    over = dict(max_rows=hints[0], max_kv=hints[1])
+    try:
+        ptts_paged.attention = lambda *a, **k: real(*a, **{**k, **over})
+        ptts_paged.attention_workspace = lambda *a, **k: query(*a, **{**k, **over})
+        for lens in ([(300, 70), (0, 1), (900, 2)], [(2500, 1), (40, 1)]):
+            for window, sinks in ((0, 0), (130, 9)):
+                _compare(*_attend(lens, 4, 2, 64, 16, kind, kind, window, sinks), kind, 64)
+    finally:
+        ptts_paged.attention, ptts_paged.attention_workspace = real, query

@@ -183,3 +183,14 @@ def test_free_pages_and_reset_beside_steps(eng):
     assert not errors and seen <= set(range(0, 41, 2)) and a.free_pages() == 0 and b.free_pages() == 40
     a.close()
     b.close()
+
+
+def test_the_codec_beside_a_paged_lm(eng):
+    """A paged state decodes as a fixed one does."""
+    rng = np.random.default_rng(9)
+    fixed, paged = eng.state(1), eng.paged_state(1, pages=4)
+    z = (rng.standard_normal((6, eng.latent)) * 0.7).astype(np.float32)
+    for part in (z[:2], z[2:]):
+        np.testing.assert_array_equal(eng.mimi_decode(paged, part[None]), eng.mimi_decode(fixed, part[None]))
+    fixed.close()
+    paged.close()
