@@ -165,6 +165,7 @@ public:
     const PagedOptions opt;
 
 private:
+    long long pages_of(long long rows) const { return (rows + opt.page_size - 1) / opt.page_size; }
     void release(int page);
     void drop(int slot);
     template <typename F> void behind_window(int slot, int length, F&& take);

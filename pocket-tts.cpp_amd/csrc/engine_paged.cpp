@@ -84,7 +84,7 @@ void PagedCache::check_room(int slot, int length, int rows, int chunk) const {
     for (int done = 0; done < rows; done += chunk) {
         const long long low = opt.window ? static_cast<long long>(length) + done - opt.window + 1 : 0, n = std::min(chunk, rows - done);
         for (; dead < have && (dead + 1) * opt.page_size <= low; ++dead) free += dead >= static_cast<long long>(held[slot].size()) || uses[held[slot][dead]] == 1;
-        const long long need = (length + done + n + opt.page_size - 1) / opt.page_size - have;
+        const long long need = std::max(0ll, pages_of(length + done + n) - have);
         if (need > free) throw std::runtime_error("the pool has " + std::to_string(free_pages.size()) + " free pages, too few for " + std::to_string(rows) + " rows");
         free -= need;
         have += need;
@@ -97,7 +97,7 @@ void PagedCache::plan(int slot0, int nb, int rows, const int* pos, hipStream_t s
     long long need = 0, back = 0;              // pages taken; pages that come back, those shared between these slots once
     for (int i = 0; i < nb; ++i) {
         if (pos[i] + static_cast<long long>(rows) > opt.max_context) throw std::runtime_error("LM context exceeds max_context");
-        need += (pos[i] + rows + opt.page_size - 1) / opt.page_size - static_cast<int>(held[slot0 + i].size());
+        need += std::max(0ll, pages_of(pos[i] + rows) - static_cast<long long>(held[slot0 + i].size()));
     }
     for (int i = 0; i < nb; ++i) behind_window(slot0 + i, pos[i], [&](int page) { back += --uses[page] == 0; });
     for (int i = 0; i < nb; ++i) behind_window(slot0 + i, pos[i], [&](int page) { ++uses[page]; });
@@ -120,14 +120,16 @@ void PagedCache::plan(int slot0, int nb, int rows, const int* pos, hipStream_t s
         host[i] = pos[i];
         host[nb + i] = rows;
         most = std::max(most, pos[i] + rows);
+        // The plan is given every page behind the slot's rows, those too that a call which failed after its plan has left here.
         auto& h = held[slot0 + i];
-        while (static_cast<long long>(h.size()) * opt.page_size < pos[i] + rows) {
+        const long long last = pages_of(pos[i] + rows);
+        while (static_cast<long long>(h.size()) < last) {
             const int page = free_pages.back();
             free_pages.pop_back();
             uses[page] = 1;
             h.push_back(page);
-            host[2 * nb + taken++] = page;
         }
+        for (long long k = pages_of(pos[i]); k < last; ++k) host[2 * nb + taken++] = h[k];
     }
     PTTS_HIP(hipMemcpyAsync(cached, host, static_cast<size_t>(nb) * 4, hipMemcpyHostToDevice, st));
     PTTS_HIP(hipMemcpyAsync(arriving, host + nb, static_cast<size_t>(nb) * 4, hipMemcpyHostToDevice, st));
