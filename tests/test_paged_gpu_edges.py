@@ -114,3 +114,10 @@ def test_hints_that_are_wrong_change_no_results(kind, hints):
                 _compare(*_attend(lens, 4, 2, 64, 16, kind, kind, window, sinks), kind, 64)
     finally:
         ptts_paged.attention, ptts_paged.attention_workspace = real, query
+
+
+@pytest.mark.parametrize("window,sinks", [(50, 2 ** 31 - 1), (2 ** 31 - 1, 0), (2 ** 31 - 1, 2 ** 31 - 1), (1 << 30, 5), ((1 << 30) + 1, 3), (-5, 7), (1, 0)])
+@pytest.mark.parametrize("kind", ["bfloat16", "float32"])
+def test_windows_and_sinks_at_their_limits(kind, window, sinks):
+    from test_paged_gpu import _attend, _compare
+    _compare(*_attend([(300, 70), (0, 1), (900, 2)], 4, 2, 64, 16, kind, kind, window, sinks), kind, 64)
